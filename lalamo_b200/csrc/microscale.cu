@@ -1,0 +1,218 @@
+// Rows into microscaled form and back, and the residual sum with its RMS norm straight into that form (see microscaled.cuh for the layout).
+// All three read every input once and write every output once; what bounds them is memory.
+#include "microscaled.cuh"
+
+namespace lb {
+
+constexpr int kMicroscaleThreads = 256;
+constexpr int kMicroscaleUnroll = 4;   // pieces of 128 columns that sixteen lanes have in flight
+
+// codes and scales of x [rows, width].  Sixteen lanes take the 128 columns under one word of scales, eight columns each.
+template <typename T, int BITS, bool VECTOR>
+__global__ void __launch_bounds__(kMicroscaleThreads)
+microscale_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int rows, int width, int chunks) {
+    wait_for_previous_kernel();
+    allow_next_kernel();
+    constexpr int kPieces = kMicroscaleThreads / 16;
+    const long long total = static_cast<long long>(rows) * chunks;
+    const long long first = static_cast<long long>(blockIdx.x) * (kPieces * kMicroscaleUnroll) + (threadIdx.x >> 4);
+    const int column = (threadIdx.x & 15) * 8;
+    float v[kMicroscaleUnroll][8];
+#pragma unroll
+    for (int u = 0; u < kMicroscaleUnroll; ++u) {
+        const long long piece = first + u * kPieces;
+        const long long row = piece / chunks;
+        const int chunk = static_cast<int>(piece - row * chunks);
+        if (piece < total) {
+            load_eight<VECTOR>(x + row * width, chunk * 128 + column, width, v[u]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kMicroscaleUnroll; ++u) {
+        const long long piece = first + u * kPieces;
+        const long long row = piece / chunks;
+        const int chunk = static_cast<int>(piece - row * chunks);
+        uint2 code;
+        const uint32_t word = quantise_eight<BITS>(v[u], code);
+        if (piece >= total) continue;
+        const size_t at = static_cast<size_t>(piece) * 128 + column;
+        if constexpr (BITS == 8) *reinterpret_cast<uint2*>(codes + at) = code;
+        else *reinterpret_cast<uint32_t*>(codes + at / 2) = code.x;
+        if (column == 0) *reinterpret_cast<uint32_t*>(scales + scale_word(static_cast<int>(row), chunk, chunks)) = word;
+    }
+}
+
+// The values [rows, width] that codes and scales stand for, rounded once to the output's type (e4m3 and e2m1 elements times their scale are exact in
+// bfloat16 down to its subnormals).
+template <typename T, int BITS, bool VECTOR>
+__global__ void __launch_bounds__(kMicroscaleThreads)
+microscaled_values_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales, T* __restrict__ out, int rows, int width, int chunks) {
+    wait_for_previous_kernel();
+    allow_next_kernel();
+    constexpr int kPieces = kMicroscaleThreads / 16;
+    const long long total = static_cast<long long>(rows) * chunks;
+    const long long first = static_cast<long long>(blockIdx.x) * (kPieces * kMicroscaleUnroll) + (threadIdx.x >> 4);
+    const int column = (threadIdx.x & 15) * 8;
+    uint2 code[kMicroscaleUnroll];
+    int byte[kMicroscaleUnroll];
+#pragma unroll
+    for (int u = 0; u < kMicroscaleUnroll; ++u) {
+        const long long piece = first + u * kPieces;
+        if (piece >= total) break;
+        const long long row = piece / chunks;
+        const int chunk = static_cast<int>(piece - row * chunks);
+        const size_t at = static_cast<size_t>(piece) * 128 + column;
+        if constexpr (BITS == 8) code[u] = *reinterpret_cast<const uint2*>(codes + at);
+        else code[u].x = *reinterpret_cast<const uint32_t*>(codes + at / 2);
+        byte[u] = scales[scale_word(static_cast<int>(row), chunk, chunks) + column / 32];
+    }
+#pragma unroll
+    for (int u = 0; u < kMicroscaleUnroll; ++u) {
+        const long long piece = first + u * kPieces;
+        if (piece >= total) break;
+        const long long row = piece / chunks;
+        const int chunk = static_cast<int>(piece - row * chunks);
+        const float scale = scale_value(byte[u]);
+        float v[8];
+        unpack_eight<BITS>(code[u], v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= scale;
+        store_eight<VECTOR>(out + row * width, chunk * 128 + column, width, v);
+    }
+}
+
+// s = x + delta; sum_out = s; y = s * rsqrt(mean(s^2) + eps) * (weight + offset), microscaled from 32 bits.  A block per row, GROUPS pieces of eight
+// columns a thread, which stay in registers between the sum of squares and the norm.  sum_out may be x: an element is read and written by one thread.
+template <typename TD, int BITS, int GROUPS, bool VECTOR>
+__global__ void __launch_bounds__(GROUPS == 4 ? 1024 : 256)
+rmsnorm_microscaled_kernel(const float* x, const TD* __restrict__ delta, float* sum_out, const float* __restrict__ weight, float offset, float eps,
+                           unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int width, int chunks) {
+    __shared__ float scratch[33];
+    wait_for_previous_kernel();
+    allow_next_kernel();
+    const int row = blockIdx.x;
+    const size_t base = static_cast<size_t>(row) * width;
+    float v[GROUPS][8];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) load_eight<VECTOR>(x + base, (threadIdx.x + g * blockDim.x) * 8, width, v[g]);
+    if (delta != nullptr) {
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            float d[8];
+            load_eight<VECTOR>(delta + base, (threadIdx.x + g * blockDim.x) * 8, width, d);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[g][i] += d[i];
+        }
+    }
+    float squares = 0.0f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        if (sum_out != nullptr) store_eight<VECTOR>(sum_out + base, (threadIdx.x + g * blockDim.x) * 8, width, v[g]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) squares += v[g][i] * v[g][i];
+    }
+    const float factor = rsqrtf(block_sum(squares, scratch) / static_cast<float>(width) + eps);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        const int column = (threadIdx.x + g * blockDim.x) * 8;
+        float w[8];
+        load_eight<VECTOR>(weight, column, width, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = column + i < width ? v[g][i] * factor * (w[i] + offset) : 0.0f;
+        uint2 code;
+        const uint32_t word = quantise_eight<BITS>(w, code);
+        if (column >= chunks * 128) continue;
+        const size_t at = static_cast<size_t>(row) * chunks * 128 + column;
+        if constexpr (BITS == 8) *reinterpret_cast<uint2*>(codes + at) = code;
+        else *reinterpret_cast<uint32_t*>(codes + at / 2) = code.x;
+        if ((column & 127) == 0) *reinterpret_cast<uint32_t*>(scales + scale_word(row, column >> 7, chunks)) = word;
+    }
+}
+
+template <typename T>
+bool rows_are_aligned(const T* rows, int width) {
+    return width % 8 == 0 && (reinterpret_cast<uintptr_t>(rows) & 15) == 0;
+}
+
+inline dim3 microscale_grid(int rows, int chunks) {
+    const long long pieces = static_cast<long long>(rows) * chunks, per_block = kMicroscaleThreads / 16 * kMicroscaleUnroll;
+    return dim3(static_cast<unsigned>((pieces + per_block - 1) / per_block));
+}
+
+template <typename T, int BITS>
+cudaError_t launch_microscale(const T* x, unsigned char* codes, unsigned char* scales, int rows, int width, cudaStream_t stream) {
+    const int chunks = (width + 127) / 128;
+    auto kernel = rows_are_aligned(x, width) ? microscale_kernel<T, BITS, true> : microscale_kernel<T, BITS, false>;
+    return launch_overlapped(kernel, microscale_grid(rows, chunks), dim3(kMicroscaleThreads), 0, stream, x, codes, scales, rows, width, chunks);
+}
+
+template <typename T, int BITS>
+cudaError_t launch_values(const unsigned char* codes, const unsigned char* scales, T* out, int rows, int width, cudaStream_t stream) {
+    const int chunks = (width + 127) / 128;
+    auto kernel = rows_are_aligned(out, width) ? microscaled_values_kernel<T, BITS, true> : microscaled_values_kernel<T, BITS, false>;
+    return launch_overlapped(kernel, microscale_grid(rows, chunks), dim3(kMicroscaleThreads), 0, stream, codes, scales, out, rows, width, chunks);
+}
+
+template <typename TD, int BITS, int GROUPS>
+cudaError_t launch_norm_groups(const float* x, const TD* delta, float* sum_out, const float* weight, float offset, float eps, unsigned char* codes,
+                               unsigned char* scales, int rows, int width, cudaStream_t stream) {
+    const int chunks = (width + 127) / 128, groups = chunks * 16;
+    const int threads = ((groups + GROUPS - 1) / GROUPS + 31) / 32 * 32;
+    const bool aligned = rows_are_aligned(x, width) && rows_are_aligned(delta, width) && rows_are_aligned(sum_out, width) && rows_are_aligned(weight, width);
+    auto kernel = aligned ? rmsnorm_microscaled_kernel<TD, BITS, GROUPS, true> : rmsnorm_microscaled_kernel<TD, BITS, GROUPS, false>;
+    return launch_overlapped(kernel, dim3(rows), dim3(threads), 0, stream, x, delta, sum_out, weight, offset, eps, codes, scales, width, chunks);
+}
+
+constexpr int kNormLargestWidth = 32768;   // 1024 threads of four pieces of eight columns
+
+template <typename TD, int BITS>
+cudaError_t launch_norm(const float* x, const TD* delta, float* sum_out, const float* weight, float offset, float eps, unsigned char* codes,
+                        unsigned char* scales, int rows, int width, cudaStream_t stream) {
+    if (width <= 2048) return launch_norm_groups<TD, BITS, 1>(x, delta, sum_out, weight, offset, eps, codes, scales, rows, width, stream);
+    if (width <= 4096) return launch_norm_groups<TD, BITS, 2>(x, delta, sum_out, weight, offset, eps, codes, scales, rows, width, stream);
+    return launch_norm_groups<TD, BITS, 4>(x, delta, sum_out, weight, offset, eps, codes, scales, rows, width, stream);
+}
+
+}  // namespace lb
+
+extern "C" {
+
+// Return codes: 0, a CUDA error, -1 for an element type, -2 for sizes that the kernels do not take.
+
+int lb_microscale(const void* x, void* codes, void* scales, int rows, int width, int bits, int dtype, cudaStream_t stream) {
+    if (rows < 0 || width < 1 || (bits != 4 && bits != 8)) return -2;
+    if (rows == 0) return 0;
+    unsigned char *c = static_cast<unsigned char*>(codes), *s = static_cast<unsigned char*>(scales);
+    LB_DISPATCH_DTYPE(dtype, {
+        const T* source = static_cast<const T*>(x);
+        return static_cast<int>(bits == 8 ? lb::launch_microscale<T, 8>(source, c, s, rows, width, stream) : lb::launch_microscale<T, 4>(source, c, s, rows, width, stream));
+    })
+}
+
+int lb_microscaled_values(const void* codes, const void* scales, void* out, int rows, int width, int bits, int dtype, cudaStream_t stream) {
+    if (rows < 0 || width < 1 || (bits != 4 && bits != 8)) return -2;
+    if (rows == 0) return 0;
+    const unsigned char *c = static_cast<const unsigned char*>(codes), *s = static_cast<const unsigned char*>(scales);
+    LB_DISPATCH_DTYPE(dtype, {
+        T* destination = static_cast<T*>(out);
+        return static_cast<int>(bits == 8 ? lb::launch_values<T, 8>(c, s, destination, rows, width, stream) : lb::launch_values<T, 4>(c, s, destination, rows, width, stream));
+    })
+}
+
+// delta (may be null) has the type `dtype`; sum_out may be null, or x.
+int lb_rmsnorm_microscaled(const float* x, const void* delta, float* sum_out, const float* weight, float offset, float eps, void* codes, void* scales, int rows,
+                           int width, int bits, int dtype, cudaStream_t stream) {
+    if (rows < 0 || width < 1 || width > lb::kNormLargestWidth || (bits != 4 && bits != 8)) return -2;
+    if (rows == 0) return 0;
+    unsigned char *c = static_cast<unsigned char*>(codes), *s = static_cast<unsigned char*>(scales);
+    LB_DISPATCH_DTYPE(dtype, {
+        const T* d = static_cast<const T*>(delta);
+        return static_cast<int>(bits == 8 ? lb::launch_norm<T, 8>(x, d, sum_out, weight, offset, eps, c, s, rows, width, stream)
+                                          : lb::launch_norm<T, 4>(x, d, sum_out, weight, offset, eps, c, s, rows, width, stream));
+    })
+}
+
+}  // extern "C"

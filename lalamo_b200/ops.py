@@ -20,7 +20,7 @@ import torch
 
 from . import native
 
-__all__ = ["BiasedSum", "ExpertSum", "KernelError", "ResidualStreams", "ResidualTerm", "TermSum", "ScaledSum", "SlicedSum", "StreamWrite", "dtype_code", "launch_count", "reset_launch_count"]
+__all__ = ["BiasedSum", "ExpertSum", "KernelError", "Microscaled", "ResidualStreams", "ResidualTerm", "TermSum", "ScaledSum", "SlicedSum", "StreamWrite", "dtype_code", "launch_count", "reset_launch_count"]
 
 
 class KernelError(RuntimeError):
@@ -2531,6 +2531,187 @@ def gated_linear(x: torch.Tensor, up_gate: torch.Tensor, activation: str, status
         return linear_tcgen05(x, up_gate, "gated", activation=activation, status=status, limit=limit)
     fused = linear(x, up_gate, status=status)
     gated_activation(fused.sum() if isinstance(fused, SlicedSum) else fused, out, activation, limit)
+    return out
+
+
+# --------------------------------------------------------------------------- microscaled rows
+@dataclass(slots=True)
+class Microscaled:
+    """Rows of ``width`` numbers in the OCP microscaling formats: elements of 8 bits (e4m3) or 4 (e2m1), every 32 columns of a row
+    under a power of two.  With ``padded`` the width made up to whole 128s:
+
+    * ``codes``: uint8 ``[rows, padded * bits / 8]``, of 4-bit elements the even column in the lower half of its byte; columns past the
+      width hold zeros;
+    * ``scales``: uint8 ``[ceil(rows / 128), padded / 128, 512]``; a byte ``b`` stands for ``2^(b - 127)``, 255 for "not a number".
+      That of row ``r`` and columns ``32 c`` to ``32 c + 31`` is byte ``(r % 32) * 16 + (r % 128) // 32 * 4 + c % 4`` of tile
+      ``[r // 128, c // 4]``; blocks past the width have any scale that is a number, rows past the last one anything.
+
+    :func:`microscale` and :func:`rmsnorm_microscaled` make them, :func:`linear_microscaled` and :func:`gated_linear_microscaled` read them;
+    :meth:`values` gives the numbers back."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    width: int
+    bits: int
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((self.codes.shape[0], self.width))
+
+    @classmethod
+    def empty(cls, rows: int, width: int, bits: int, device: torch.device) -> "Microscaled":
+        """Room for ``rows`` rows, not yet written."""
+        chunks = -(-width // 128)
+        codes = torch.empty((rows, chunks * 16 * bits), dtype=torch.uint8, device=device)
+        return cls(codes, torch.empty((-(-rows // 128), chunks, 512), dtype=torch.uint8, device=device), width, bits)
+
+    def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The numbers, ``[rows, width]``: exact in float32, and in bfloat16 down to its subnormals."""
+        _check_microscaled(self, "microscaled_values")
+        code = dtype_code(dtype)
+        rows = self.codes.shape[0]
+        out = torch.empty((rows, self.width), dtype=dtype, device=self.codes.device)
+        if rows:
+            _done(_lib().lb_microscaled_values(self.codes, self.scales, out, rows, self.width, self.bits, code, _stream()), "microscaled_values")
+        return out
+
+
+MICROSCALED_BITS = (4, 8)
+MICROSCALED_NORM_LARGEST_WIDTH = 32768
+
+
+def _check_microscaled(rows: Microscaled, what: str) -> int:
+    """Refuses what is not microscaled rows on the current device as :class:`Microscaled` describes them; returns the width in 128s."""
+    codes, scales, bits = rows.codes, rows.scales, rows.bits
+    if bits != 8 and bits != 4:
+        raise KernelError(f"{what}: elements have 4 or 8 bits, not {bits}")
+    chunks = -(-rows.width // 128)
+    if rows.width < 1 or codes.dim() != 2 or codes.shape[1] != chunks * 16 * bits:
+        raise KernelError(f"{what}: codes of shape {tuple(codes.shape)} are not rows of {rows.width} elements of {bits} bits, made up to whole 128s")
+    if scales.shape != (-(-codes.shape[0] // 128), chunks, 512):
+        raise KernelError(f"{what}: scales of shape {tuple(scales.shape)} do not belong to {codes.shape[0]} rows of {rows.width} elements")
+    if not (codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_contiguous() and scales.is_contiguous()):
+        raise KernelError(f"{what}: codes and scales are contiguous and of uint8")
+    _check_here(what, codes, scales)
+    if codes.data_ptr() % 32 or scales.data_ptr() % 16:
+        raise KernelError(f"{what}: codes start on 32 bytes and scales on 16")
+    return chunks
+
+
+def _check_here(what: str, *tensors: torch.Tensor) -> None:
+    """Refuses tensors that do not lie on the current device, on whose stream the kernel is launched."""
+    device = _current_device() if tensors[0].is_cuda else -1
+    for tensor in tensors:
+        if not tensor.is_cuda:
+            raise KernelError(f"{what}: all tensors must live on a CUDA device (there is no CPU path)")
+        if tensor.get_device() != device:
+            raise KernelError(f"{what}: a tensor lies on device {tensor.get_device()}, the current device is {device}")
+
+
+def microscale(x: torch.Tensor, bits: int = 8) -> Microscaled:
+    """Rows ``x`` (bfloat16 or float32, ``[rows, width]``) in microscaled form.  The scale of a block of 32 columns is
+    ``2^(floor(log2(max |x|)) - e)`` with the exponent ``e`` of the format's largest element (8 of 448, 2 of 6), at least ``2^-127``; its elements
+    are ``x / scale`` to the nearest, ties to even, and the largest element for what is larger.  A block that holds a NaN or an infinity becomes
+    NaN as a whole."""
+    if bits not in MICROSCALED_BITS:
+        raise KernelError(f"microscale: elements have 4 or 8 bits, not {bits}")
+    _check(x, "x")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise KernelError(f"microscale: x must be [rows, width], got {tuple(x.shape)}")
+    code = dtype_code(x.dtype)
+    _check_here("microscale", x)
+    rows, width = x.shape
+    out = Microscaled.empty(rows, width, bits, x.device)
+    if rows:
+        _done(_lib().lb_microscale(x, out.codes, out.scales, rows, width, bits, code, _stream()), "microscale")
+    return out
+
+
+def rmsnorm_microscaled(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta: torch.Tensor | None = None, sum_out: torch.Tensor | None = None,
+                        scale_offset: float = 0.0, bits: int = 8) -> Microscaled:
+    """``rms_norm(x + delta) * (weight + scale_offset)`` in microscaled form, from 32 bits in one rounding (the scales' and elements' rule is
+    :func:`microscale`'s).  ``x`` is the 32-bit residual stream ``[rows, width]``, ``delta`` (bfloat16 or float32) what is added to it first;
+    ``sum_out`` (float32; it may be ``x`` itself) receives the sum.  Rows of up to 32,768 columns."""
+    if bits not in MICROSCALED_BITS:
+        raise KernelError(f"rmsnorm_microscaled: elements have 4 or 8 bits, not {bits}")
+    _check(x, "x", torch.float32)
+    _check(weight, "weight", torch.float32)
+    if x.dim() != 2 or not 1 <= x.shape[1] <= MICROSCALED_NORM_LARGEST_WIDTH:
+        raise KernelError(f"rmsnorm_microscaled: x must be [rows, width] with a width of 1 to {MICROSCALED_NORM_LARGEST_WIDTH}, got {tuple(x.shape)}")
+    rows, width = x.shape
+    if weight.dim() != 1 or weight.shape[0] != width:
+        raise KernelError("rmsnorm_microscaled: weight must have one element per column")
+    here = [x, weight]
+    code = 0
+    if delta is not None:
+        _check(delta, "delta")
+        if delta.shape != x.shape:
+            raise KernelError("rmsnorm_microscaled: delta and x differ in shape")
+        code = dtype_code(delta.dtype)
+        here.append(delta)
+    if sum_out is not None:
+        _check(sum_out, "sum_out", torch.float32)
+        if sum_out.shape != x.shape:
+            raise KernelError("rmsnorm_microscaled: sum_out and x differ in shape")
+        if sum_out.data_ptr() != x.data_ptr() and _overlap(sum_out, x) or delta is not None and _overlap(sum_out, delta) or _overlap(sum_out, weight):
+            raise KernelError("rmsnorm_microscaled: sum_out may be x, but not overlap it otherwise, nor delta or weight")
+        here.append(sum_out)
+    _check_here("rmsnorm_microscaled", *here)
+    out = Microscaled.empty(rows, width, bits, x.device)
+    if rows:
+        _done(_lib().lb_rmsnorm_microscaled(x, delta, sum_out, weight, scale_offset, eps, out.codes, out.scales, rows, width, bits, code, _stream()), "rmsnorm_microscaled")
+    return out
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share bytes."""
+    first, second = a.data_ptr(), b.data_ptr()
+    return first < second + b.nbytes and second < first + a.nbytes
+
+
+def linear_microscaled(x: Microscaled, weight: Microscaled, out_dtype: torch.dtype = torch.bfloat16, status: torch.Tensor | None = None) -> torch.Tensor:
+    """``x @ weight.T`` of the values that microscaled rows stand for: ``x`` in 8 or 4 bits, ``weight`` ``[rows, width]`` in 4; sums of 32 bits, rounded once
+    to bfloat16 or handed out as float32.  ``status``: the int32 word in which the kernel reports a wait that gave up."""
+    chunks = _check_microscaled(x, "linear_microscaled")
+    _check_microscaled(weight, "linear_microscaled")
+    if weight.bits != 4 or weight.width != x.width:
+        raise KernelError(f"linear_microscaled: a weight of {weight.width} columns in {weight.bits} bits for rows of {x.width} (the widths must agree, weights have 4 bits)")
+    code = dtype_code(out_dtype)
+    if status is not None:
+        _check(status, "status", torch.int32)
+    tokens, rows = x.codes.shape[0], weight.codes.shape[0]
+    out = torch.empty((tokens, rows), dtype=out_dtype, device=x.codes.device)
+    if tokens and rows:
+        code = _lib().lb_gemm_microscaled(x.codes, x.scales, weight.codes, weight.scales, out, tokens, rows, chunks, x.bits, 1 if code == 0 else 0, status, _stream())
+        if code == -5:
+            raise KernelError("linear_microscaled: the driver gave no tensor map (cuTensorMapEncodeTiled)")
+        _done(code, "gemm_microscaled")
+    return out
+
+
+def gated_linear_microscaled(x: Microscaled, up: Microscaled, gate: Microscaled, activation: str, limit: float = 0.0, status: torch.Tensor | None = None) -> Microscaled:
+    """``(x @ up.T) * act(x @ gate.T)`` of microscaled rows (8 or 4 bits) and weights (4 bits, ``[hidden, width]`` each), in 8 bits: sums, activation and product
+    in 32 bits, then :func:`microscale`'s rule.  ``limit``: of the ``"sigmoid_limit"`` activation.  ``status`` as in :func:`linear_microscaled`."""
+    chunks = _check_microscaled(x, "gated_linear_microscaled")
+    _check_microscaled(up, "gated_linear_microscaled")
+    _check_microscaled(gate, "gated_linear_microscaled")
+    if activation not in _ACTIVATIONS:
+        raise KernelError(f"unknown activation {activation!r}; known: {sorted(_ACTIVATIONS)}")
+    if up.bits != 4 or gate.bits != 4 or up.width != x.width or up.shape != gate.shape:
+        raise KernelError(f"gated_linear_microscaled: weights of {tuple(up.shape)} in {up.bits} bits and {tuple(gate.shape)} in {gate.bits} for rows of {x.width} "
+                          "(both must be [hidden, width] in 4 bits)")
+    if status is not None:
+        _check(status, "status", torch.int32)
+    tokens, hidden = x.codes.shape[0], up.codes.shape[0]
+    if not hidden:
+        raise KernelError("gated_linear_microscaled: the weights have no rows")
+    out = Microscaled.empty(tokens, hidden, 8, x.codes.device)
+    if tokens:
+        code = _lib().lb_gated_microscaled(x.codes, x.scales, up.codes, up.scales, gate.codes, gate.scales, out.codes, out.scales, tokens, hidden, chunks, x.bits,
+                                           _ACTIVATIONS[activation], limit, status, _stream())
+        if code == -5:
+            raise KernelError("gated_linear_microscaled: the driver gave no tensor map (cuTensorMapEncodeTiled)")
+        _done(code, "gated_microscaled")
     return out
 
 
