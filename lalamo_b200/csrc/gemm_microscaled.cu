@@ -416,6 +416,240 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Walk::kColumns) : "memory");
 }
 
+// ---------------------------------------------------------------------------------------------
+// The same where the tiles alone would leave most multiprocessors idle (few tokens, or few of both): the CTAs of a cluster share a tile's K, and the sums of
+// their parts meet in shared memory.  Every CTA then adds up the tokens rank, rank + S, ... of the tile, part after part in the parts' order, and sends
+// them off; a second launch and a trip of the parts through memory are saved.
+// ---------------------------------------------------------------------------------------------
+constexpr int kMsSplitThreads = 256;   // producer, issuer, scales of a gated product, one idle, four that read tensor memory; all of them add up
+constexpr int kMsLargestSplit = 8;     // CTAs of a cluster
+constexpr int kMsSplitStages = 11;     // of the ring, at most
+constexpr int kMsSplitShared = kMsSharedLimit - 1024;   // beside the variables
+
+template <int BITS, int BN>
+struct MsSplit {
+    static constexpr int kScaleColumns = 4 * MsShape<BITS, BN>::kChunks * 2;
+    static constexpr int kColumns = BN + kScaleColumns <= 32 ? 32 : BN + kScaleColumns <= 64 ? 64 : BN + kScaleColumns <= 128 ? 128 : 256;
+    static constexpr int kPartBytes = BN * kMsRows * 4;   // the parts' sums, where the ring was
+    static constexpr int kSlack = 1024 + 256;             // alignment and barriers
+    static constexpr int kRoom = (kMsSplitShared - kSlack) / MsShape<BITS, BN>::kStageBytes;
+    static constexpr int kMostStages = kRoom < kMsSplitStages ? kRoom : kMsSplitStages;
+    static int bytes(int stages) {
+        const int ring = stages * MsShape<BITS, BN>::kStageBytes;
+        return (ring > kPartBytes ? ring : kPartBytes) + kSlack;
+    }
+};
+
+__device__ __forceinline__ float load_cluster(uint32_t address) {
+    float value;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(value) : "r"(address) : "memory");
+    return value;
+}
+
+template <int BITS, int BN, bool GATED>
+__global__ void __launch_bounds__(kMsSplitThreads)
+gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_gate, const __grid_constant__ CUtensorMap map_x, const MsParams p,
+                              int splits, int stages_per_split, int ring_stages) {
+    using Shape = MsShape<BITS, BN>;
+    using Split = MsSplit<BITS, BN>;
+    static_assert(BN <= 128, "one tile of scales for the tokens");
+    extern __shared__ unsigned char raw_shared[];
+    __shared__ uint64_t barriers[2 * kMsSplitStages + 1];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int failed;
+    unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_shared) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint64_t* full = barriers;
+    uint64_t* empty = barriers + kMsSplitStages;
+    uint64_t* accumulated = barriers + 2 * kMsSplitStages;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kRowsPerTile = GATED ? kMsRows / 2 : kMsRows;
+    const int rank = static_cast<int>(blockIdx.x) % splits;   // the cluster's CTAs are neighbours
+    const int row0 = static_cast<int>(blockIdx.x) / splits * kRowsPerTile, token0 = blockIdx.y * BN;
+    const int num_stages = (p.chunks + Shape::kChunks - 1) / Shape::kChunks;
+    const int first_stage = rank * stages_per_split, count = min(stages_per_split, num_stages - first_stage);   // at least one: the launcher sees to it
+    auto chunks_of = [&](int stage) { return min(Shape::kChunks, p.chunks - stage * Shape::kChunks); };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < ring_stages; ++s) {
+            barrier_init(&full[s], GATED ? 2 : 1);
+            barrier_init(&empty[s], 1);
+        }
+        barrier_init(accumulated, 1);
+        failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(&tmem_slot)), "r"(Split::kColumns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = tmem_slot;
+    const uint32_t tmem_w_scales = tmem_base + BN, tmem_x_scales = tmem_w_scales + 4 * Shape::kChunks;
+    wait_for_previous_kernel();   // the weights may be what it has made
+    allow_next_kernel();
+
+    if (warp == 0 && lane == 0) {
+        const unsigned char* w_scales = p.w_scales + static_cast<size_t>(row0 / 128) * p.chunks * kScaleTileBytes;
+        const unsigned char* x_scales = p.x_scales + static_cast<size_t>(token0 / 128) * p.chunks * kScaleTileBytes;
+        for (int i = 0, s = 0, round = 0; i < count; ++i) {
+            if (round > 0 && !barrier_wait(&empty[s], (round - 1) & 1)) {
+                atomicExch(&failed, 1);
+                break;
+            }
+            const int stage = first_stage + i, column = stage * 128, chunk = stage * Shape::kChunks;
+            unsigned char* at = ring + s * Shape::kStageBytes;
+            const uint32_t scale_bytes = static_cast<uint32_t>(chunks_of(stage) * kScaleTileBytes);
+            barrier_expect(&full[s], Shape::kWCounted + Shape::kXBytes + (GATED ? 1u : 2u) * scale_bytes);
+            tma_load_2d(at, &map_w, column, row0, &full[s]);
+            if constexpr (GATED) tma_load_2d(at + Shape::kWBytes / 2, &map_gate, column, row0, &full[s]);
+            tma_load_2d(at + Shape::kWBytes, &map_x, column, token0, &full[s]);
+            at += Shape::kWBytes + Shape::kXBytes;
+            if constexpr (!GATED) bulk_load(at, w_scales + static_cast<size_t>(chunk) * kScaleTileBytes, scale_bytes, &full[s]);
+            bulk_load(at + Shape::kWScaleBytes, x_scales + static_cast<size_t>(chunk) * kScaleTileBytes, scale_bytes, &full[s]);
+            if (++s == ring_stages) s = 0, ++round;
+        }
+    } else if (warp == 1 && lane == 0) {
+        const uint32_t idesc = microscaled_descriptor<BITS>(BN);
+        const uint32_t x_column = tmem_x_scales + static_cast<uint32_t>((token0 & 127) >> 5);
+        bool ok = true;
+        for (int i = 0, s = 0, round = 0; i < count; ++i) {
+            if (!barrier_wait(&full[s], round & 1)) {
+                atomicExch(&failed, 1);
+                ok = false;
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            unsigned char* at = ring + s * Shape::kStageBytes;
+            const unsigned char* scales = at + Shape::kWBytes + Shape::kXBytes;
+            const int here = chunks_of(first_stage + i);
+#pragma unroll
+            for (int c = 0; c < Shape::kChunks; ++c) {
+                if (c >= here) break;
+                copy_scales(tmem_w_scales + 4 * c, scales + c * kScaleTileBytes);
+                copy_scales(tmem_x_scales + 4 * c, scales + Shape::kWScaleBytes + c * kScaleTileBytes);
+            }
+            const uint64_t desc_w = tile_descriptor(at), desc_x = tile_descriptor(at + Shape::kWBytes);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int c = product_chunk<BITS>(k);
+                if (c >= here) break;
+                mma_microscaled<BITS>(tmem_base, desc_w + 2 * k, desc_x + 2 * k, idesc | product_scales<BITS>(k), tmem_w_scales + 4 * c, x_column + 4 * c, i > 0 || k > 0);
+            }
+            mma_commit(&empty[s]);
+            if (++s == ring_stages) s = 0, ++round;
+        }
+        if (ok) mma_commit(accumulated);
+    } else if (GATED && warp == 2) {
+        // as in the walking kernel
+        const size_t offset = static_cast<size_t>(row0 / 128) * p.chunks * kScaleTileBytes + lane * 16 + ((row0 & 64) >> 3);
+        bool ok = true;
+        for (int first = 0, s = 0, round = 0; first < count && ok; first += 4) {
+            uint2 up[4][Shape::kChunks], gate[4][Shape::kChunks];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int c = 0; c < Shape::kChunks; ++c) {
+                    const int chunk = (first_stage + first + i) * Shape::kChunks + c;
+                    up[i][c] = gate[i][c] = make_uint2(0u, 0u);
+                    if (chunk < p.chunks) {
+                        up[i][c] = *reinterpret_cast<const uint2*>(p.w_scales + offset + static_cast<size_t>(chunk) * kScaleTileBytes);
+                        gate[i][c] = *reinterpret_cast<const uint2*>(p.gate_scales + offset + static_cast<size_t>(chunk) * kScaleTileBytes);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (first + i >= count) break;
+                ok = __all_sync(0xffffffffu, round == 0 || barrier_wait(&empty[s], (round - 1) & 1));
+                if (!ok) {
+                    atomicExch(&failed, 1);
+                    break;
+                }
+                unsigned char* at = ring + s * Shape::kStageBytes + Shape::kWBytes + Shape::kXBytes + lane * 16;
+#pragma unroll
+                for (int c = 0; c < Shape::kChunks; ++c) *reinterpret_cast<uint4*>(at + c * kScaleTileBytes) = make_uint4(up[i][c].x, up[i][c].y, gate[i][c].x, gate[i][c].y);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) barrier_arrive(&full[s]);
+                if (++s == ring_stages) s = 0, ++round;
+            }
+        }
+    } else if (warp >= 4) {
+        const int quarter = warp & 3;
+        const bool ok = __all_sync(0xffffffffu, barrier_wait(accumulated, 0));
+        if (ok) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            float* part = reinterpret_cast<float*>(ring) + quarter * 32 + lane;
+#pragma unroll 1
+            for (int column = 0; column < BN; column += 16) {
+                if (token0 + column >= p.tokens) break;
+                uint32_t v[16];
+                tmem_load_16(tmem_base + static_cast<uint32_t>(column) + (static_cast<uint32_t>(quarter * 32) << 16), v);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) part[(column + i) * kMsRows] = __uint_as_float(v[i]);
+            }
+        } else if (lane == 0) {
+            atomicExch(&failed, 1);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncwarp();
+    cluster_sync();   // all parts are there, or some CTA has failed and says so below
+    const int tokens_here = min(BN, p.tokens - token0);
+    const uint32_t part = smem_address(ring);
+    uint32_t parts[kMsLargestSplit];
+#pragma unroll
+    for (int q = 0; q < kMsLargestSplit; ++q) {
+        parts[q] = part;
+        if (q < splits) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(parts[q]) : "r"(part), "r"(q));
+    }
+    auto sum_of = [&](int token, int row) {
+        const uint32_t offset = static_cast<uint32_t>(token * kMsRows + row) * 4u;
+        float v[kMsLargestSplit], sum = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kMsLargestSplit; ++q) v[q] = q < splits ? load_cluster(parts[q] + offset) : 0.0f;
+#pragma unroll
+        for (int q = 0; q < kMsLargestSplit; ++q) sum = q == 0 ? v[0] : q < splits ? sum + v[q] : sum;
+        return sum;
+    };
+    if constexpr (!GATED) {
+        const int row = threadIdx.x & 127;
+        if (row0 + row < p.n) {
+#pragma unroll 2
+            for (int t = rank + (threadIdx.x >> 7) * splits; t < tokens_here; t += 2 * splits) {
+                const float sum = sum_of(t, row);
+                const size_t at = static_cast<size_t>(token0 + t) * p.n + row0 + row;
+                if (p.out_is_float) static_cast<float*>(p.out)[at] = sum;
+                else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(sum);
+            }
+        }
+    } else {
+        // A warp takes a block of 32 channels of a token at a time.
+        const int half = warp & 1, channel = half * 32 + lane;
+        const bool exists = row0 + channel < p.n;
+        for (int t = rank + (warp >> 1) * splits; t < tokens_here; t += 4 * splits) {
+            const float u = sum_of(t, channel), g = sum_of(t, kMsRows / 2 + channel);
+            const float h = exists ? ms_up_side(u, p.activation, p.limit) * ms_gate_side(g, p.activation, p.limit) : 0.0f;
+            const int byte = scale_byte<8>(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu));
+            const float scaled = byte == kNoNumber ? 0.0f : h * scale_inverse(byte);
+            const int token = token0 + t, block = row0 / 32 + half;
+            static_cast<unsigned char*>(p.out)[static_cast<size_t>(token) * p.out_chunks * 128 + row0 + channel] = static_cast<unsigned char>(pack_e4m3(scaled, 0.0f, 0.0f, 0.0f));
+            if (lane == 0) p.out_scales[scale_word(token, block >> 2, p.out_chunks) + (block & 3)] = static_cast<unsigned char>(byte);
+        }
+    }
+    __syncthreads();
+    if (failed) {
+        if (threadIdx.x == 0) report_error(p.status, kWaitTimeout);
+        for (int spin = 0; spin < 2000; ++spin) __nanosleep(1000);
+        __syncthreads();
+    }
+    cluster_sync();   // nobody leaves while another still reads its part
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Split::kColumns) : "memory");
+}
+
 // Codes as boxes of [box_rows, 128 bytes of shared memory] with 128-byte swizzle; `spread`: 4-bit elements to 16 in 16 bytes (boxes of 128 elements),
 // else the bytes as they are.  What lies outside reads as zero.
 static bool make_codes_map(CUtensorMap* map, const void* codes, int rows, int row_bytes, int box_rows, bool spread) {
@@ -468,10 +702,49 @@ int launch_microscaled(const void* x, const void* w, const void* gate, MsParams 
     return static_cast<int>(launch_overlapped(kernel, dim3(tiles < sms ? tiles : sms), dim3(kMsThreads), MsWalk<BITS, BN>::kBytes, stream, map_w, map_gate, map_x, map_out, p));
 }
 
+template <int BITS, int BN, bool GATED>
+int launch_microscaled_split(const void* x, const void* w, const void* gate, MsParams p, cudaStream_t stream) {
+    CUtensorMap map_w, map_gate, map_x;
+    const int w_bytes = p.chunks * 64, x_bytes = p.chunks * 16 * BITS;
+    if (!make_codes_map(&map_w, w, p.n, w_bytes, GATED ? kMsRows / 2 : kMsRows, BITS == 8) || !make_codes_map(&map_x, x, p.tokens, x_bytes, BN, false)) return -5;
+    map_gate = map_w;
+    if (GATED && !make_codes_map(&map_gate, gate, p.n, w_bytes, kMsRows / 2, BITS == 8)) return -5;
+    const int row_tiles = GATED ? p.out_chunks * 2 : (p.n + kMsRows - 1) / kMsRows, token_tiles = (p.tokens + BN - 1) / BN, sms = multiprocessor_count();
+    const int stages = (p.chunks + MsShape<BITS, BN>::kChunks - 1) / MsShape<BITS, BN>::kChunks;
+    const int wanted = max(1, min(min(sms / (row_tiles * token_tiles), kMsLargestSplit), stages));
+    const int per_split = (stages + wanted - 1) / wanted, splits = (stages + per_split - 1) / per_split;   // each has a stage at least
+    int ring = min(per_split, MsSplit<BITS, BN>::kMostStages);
+    // more CTAs than multiprocessors: half the ring, so that two share one
+    if (row_tiles * token_tiles * splits > sms) ring = min(ring, (kMsSplitShared / 2 - 1024 - MsSplit<BITS, BN>::kSlack) / MsShape<BITS, BN>::kStageBytes);
+    auto kernel = gemm_microscaled_split_kernel<BITS, BN, GATED>;
+    static OncePerDevice configured;
+    if (allow_shared_memory(configured, kernel, kMsSplitShared) != cudaSuccess) return static_cast<int>(cudaGetLastError());
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(row_tiles * splits, token_tiles);
+    config.blockDim = dim3(kMsSplitThreads);
+    config.dynamicSmemBytes = MsSplit<BITS, BN>::bytes(ring);
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeClusterDimension;
+    attributes[0].val.clusterDim.x = splits;
+    attributes[0].val.clusterDim.y = 1;
+    attributes[0].val.clusterDim.z = 1;
+    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[1].val.programmaticStreamSerializationAllowed = overlap_launches() ? 1 : 0;
+    config.attrs = attributes;
+    config.numAttrs = 2;
+    return static_cast<int>(cudaLaunchKernelEx(&config, kernel, map_w, map_gate, map_x, p, splits, per_split, ring));
+}
+
+// Which kernel: tiles of 128 rows x 192 tokens that fill the multiprocessors are walked; fewer are cut along K.
 template <int BITS, bool GATED>
 int launch_microscaled_tiles(const void* x, const void* w, const void* gate, const MsParams& p, cudaStream_t stream) {
-    if (p.tokens <= 64) return launch_microscaled<BITS, 64, GATED>(x, w, gate, p, stream);
-    if (p.tokens <= 128) return launch_microscaled<BITS, 128, GATED>(x, w, gate, p, stream);
+    const int row_tiles = GATED ? p.out_chunks * 2 : (p.n + kMsRows - 1) / kMsRows, sms = multiprocessor_count();
+    if (p.tokens <= 16) return launch_microscaled_split<BITS, 16, GATED>(x, w, gate, p, stream);
+    if (p.tokens <= 32) return launch_microscaled_split<BITS, 32, GATED>(x, w, gate, p, stream);
+    if (p.tokens <= 64) return launch_microscaled_split<BITS, 64, GATED>(x, w, gate, p, stream);
+    if (p.tokens <= 128 || row_tiles * ((p.tokens + 127) / 128) <= sms / 2) return launch_microscaled_split<BITS, 128, GATED>(x, w, gate, p, stream);
+    if (row_tiles * ((p.tokens + 127) / 128) <= sms) return launch_microscaled<BITS, 128, GATED>(x, w, gate, p, stream);
     return launch_microscaled<BITS, 192, GATED>(x, w, gate, p, stream);
 }
 

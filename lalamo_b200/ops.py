@@ -2535,7 +2535,6 @@ def gated_linear(x: torch.Tensor, up_gate: torch.Tensor, activation: str, status
 
 
 # --------------------------------------------------------------------------- microscaled rows
-@dataclass(slots=True)
 class Microscaled:
     """Rows of ``width`` numbers in the OCP microscaling formats: elements of 8 bits (e4m3) or 4 (e2m1), every 32 columns of a row
     under a power of two.  With ``padded`` the width made up to whole 128s:
@@ -2547,32 +2546,77 @@ class Microscaled:
       ``[r // 128, c // 4]``; blocks past the width have any scale that is a number, rows past the last one anything.
 
     :func:`microscale` and :func:`rmsnorm_microscaled` make them, :func:`linear_microscaled` and :func:`gated_linear_microscaled` read them;
-    :meth:`values` gives the numbers back."""
+    :meth:`values` gives the numbers back.  Tensors that do not fit this are refused here."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
-    width: int
-    bits: int
+    __slots__ = ("_codes", "_scales", "_store", "bits", "chunks", "device_index", "rows", "width")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, width: int, bits: int) -> None:
+        if bits != 8 and bits != 4:
+            raise KernelError(f"Microscaled: elements have 4 or 8 bits, not {bits}")
+        chunks = -(-width // 128)
+        if width < 1 or codes.dim() != 2 or codes.shape[1] != chunks * 16 * bits:
+            raise KernelError(f"Microscaled: codes of shape {tuple(codes.shape)} are not rows of {width} elements of {bits} bits, made up to whole 128s")
+        rows = codes.shape[0]
+        if scales.shape != (-(-rows // 128), chunks, 512):
+            raise KernelError(f"Microscaled: scales of shape {tuple(scales.shape)} do not belong to {rows} rows of {width} elements")
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or not codes.is_contiguous() or not scales.is_contiguous():
+            raise KernelError("Microscaled: codes and scales are contiguous and of uint8")
+        device = codes.get_device()
+        if device < 0 or scales.get_device() != device:
+            raise KernelError("Microscaled: codes and scales must live on one CUDA device (there is no CPU path)")
+        if codes.data_ptr() % 32 or scales.data_ptr() % 16:
+            raise KernelError("Microscaled: codes start on 32 bytes and scales on 16")
+        self._codes, self._scales, self._store = codes, scales, None
+        self.rows, self.width, self.bits, self.chunks, self.device_index = rows, width, bits, chunks, device
+
+    @classmethod
+    def _empty(cls, rows: int, width: int, bits: int, like: torch.Tensor) -> "Microscaled":
+        """Room for ``rows`` rows on the device of ``like``: one allocation, the scales behind the codes (whole 64 bytes of them).  The two tensors are
+        made when somebody asks for them; two allocations and the checks above took 5 us of a call of 10."""
+        self = cls.__new__(cls)
+        chunks = -(-width // 128)
+        self._store = like.new_empty(rows * chunks * 16 * bits + -(-rows // 128) * chunks * 512, dtype=torch.uint8)
+        self._codes = self._scales = None
+        self.rows, self.width, self.bits, self.chunks, self.device_index = rows, width, bits, chunks, like.get_device()
+        return self
+
+    def _split(self) -> None:
+        row_bytes = self.chunks * 16 * self.bits
+        self._codes = self._store[: self.rows * row_bytes].view(self.rows, row_bytes)
+        self._scales = self._store[self.rows * row_bytes :].view(-(-self.rows // 128), self.chunks, 512)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._split()
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._split()
+        return self._scales
 
     @property
     def shape(self) -> torch.Size:
-        return torch.Size((self.codes.shape[0], self.width))
+        return torch.Size((self.rows, self.width))
 
-    @classmethod
-    def empty(cls, rows: int, width: int, bits: int, device: torch.device) -> "Microscaled":
-        """Room for ``rows`` rows, not yet written."""
-        chunks = -(-width // 128)
-        codes = torch.empty((rows, chunks * 16 * bits), dtype=torch.uint8, device=device)
-        return cls(codes, torch.empty((-(-rows // 128), chunks, 512), dtype=torch.uint8, device=device), width, bits)
+    def _addresses(self, what: str) -> tuple[int, int]:
+        """Of codes and scales, for a launch on the current device's stream."""
+        if self.device_index != _current_device():
+            raise KernelError(f"{what}: rows on device {self.device_index}, the current device is {_current_device()}")
+        if self._store is not None:
+            address = self._store.data_ptr()
+            return address, address + self.rows * self.chunks * 16 * self.bits
+        return self._codes.data_ptr(), self._scales.data_ptr()
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The numbers, ``[rows, width]``: exact in float32, and in bfloat16 down to its subnormals."""
-        _check_microscaled(self, "microscaled_values")
+        codes, scales = self._addresses("microscaled_values")
         code = dtype_code(dtype)
-        rows = self.codes.shape[0]
-        out = torch.empty((rows, self.width), dtype=dtype, device=self.codes.device)
-        if rows:
-            _done(_lib().lb_microscaled_values(self.codes, self.scales, out, rows, self.width, self.bits, code, _stream()), "microscaled_values")
+        out = (self._store if self._store is not None else self._codes).new_empty((self.rows, self.width), dtype=dtype)
+        if self.rows:
+            _done(_lib().lb_microscaled_values(codes, scales, out, self.rows, self.width, self.bits, code, _stream()), "microscaled_values")
         return out
 
 
@@ -2580,30 +2624,10 @@ MICROSCALED_BITS = (4, 8)
 MICROSCALED_NORM_LARGEST_WIDTH = 32768
 
 
-def _check_microscaled(rows: Microscaled, what: str) -> int:
-    """Refuses what is not microscaled rows on the current device as :class:`Microscaled` describes them; returns the width in 128s."""
-    codes, scales, bits = rows.codes, rows.scales, rows.bits
-    if bits != 8 and bits != 4:
-        raise KernelError(f"{what}: elements have 4 or 8 bits, not {bits}")
-    chunks = -(-rows.width // 128)
-    if rows.width < 1 or codes.dim() != 2 or codes.shape[1] != chunks * 16 * bits:
-        raise KernelError(f"{what}: codes of shape {tuple(codes.shape)} are not rows of {rows.width} elements of {bits} bits, made up to whole 128s")
-    if scales.shape != (-(-codes.shape[0] // 128), chunks, 512):
-        raise KernelError(f"{what}: scales of shape {tuple(scales.shape)} do not belong to {codes.shape[0]} rows of {rows.width} elements")
-    if not (codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_contiguous() and scales.is_contiguous()):
-        raise KernelError(f"{what}: codes and scales are contiguous and of uint8")
-    _check_here(what, codes, scales)
-    if codes.data_ptr() % 32 or scales.data_ptr() % 16:
-        raise KernelError(f"{what}: codes start on 32 bytes and scales on 16")
-    return chunks
-
-
 def _check_here(what: str, *tensors: torch.Tensor) -> None:
     """Refuses tensors that do not lie on the current device, on whose stream the kernel is launched."""
-    device = _current_device() if tensors[0].is_cuda else -1
+    device = _current_device()
     for tensor in tensors:
-        if not tensor.is_cuda:
-            raise KernelError(f"{what}: all tensors must live on a CUDA device (there is no CPU path)")
         if tensor.get_device() != device:
             raise KernelError(f"{what}: a tensor lies on device {tensor.get_device()}, the current device is {device}")
 
@@ -2619,11 +2643,11 @@ def microscale(x: torch.Tensor, bits: int = 8) -> Microscaled:
     if x.dim() != 2 or x.shape[1] < 1:
         raise KernelError(f"microscale: x must be [rows, width], got {tuple(x.shape)}")
     code = dtype_code(x.dtype)
-    _check_here("microscale", x)
     rows, width = x.shape
-    out = Microscaled.empty(rows, width, bits, x.device)
+    out = Microscaled._empty(rows, width, bits, x)
     if rows:
-        _done(_lib().lb_microscale(x, out.codes, out.scales, rows, width, bits, code, _stream()), "microscale")
+        codes, scales = out._addresses("microscale")
+        _done(_lib().lb_microscale(x, codes, scales, rows, width, bits, code, _stream()), "microscale")
     return out
 
 
@@ -2657,9 +2681,10 @@ def rmsnorm_microscaled(x: torch.Tensor, weight: torch.Tensor, eps: float, *, de
             raise KernelError("rmsnorm_microscaled: sum_out may be x, but not overlap it otherwise, nor delta or weight")
         here.append(sum_out)
     _check_here("rmsnorm_microscaled", *here)
-    out = Microscaled.empty(rows, width, bits, x.device)
+    out = Microscaled._empty(rows, width, bits, x)
     if rows:
-        _done(_lib().lb_rmsnorm_microscaled(x, delta, sum_out, weight, scale_offset, eps, out.codes, out.scales, rows, width, bits, code, _stream()), "rmsnorm_microscaled")
+        codes, scales = out._addresses("rmsnorm_microscaled")
+        _done(_lib().lb_rmsnorm_microscaled(x, delta, sum_out, weight, scale_offset, eps, codes, scales, rows, width, bits, code, _stream()), "rmsnorm_microscaled")
     return out
 
 
@@ -2672,17 +2697,18 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 def linear_microscaled(x: Microscaled, weight: Microscaled, out_dtype: torch.dtype = torch.bfloat16, status: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T`` of the values that microscaled rows stand for: ``x`` in 8 or 4 bits, ``weight`` ``[rows, width]`` in 4; sums of 32 bits, rounded once
     to bfloat16 or handed out as float32.  ``status``: the int32 word in which the kernel reports a wait that gave up."""
-    chunks = _check_microscaled(x, "linear_microscaled")
-    _check_microscaled(weight, "linear_microscaled")
+    codes, scales = x._addresses("linear_microscaled")
+    weight_codes, weight_scales = weight._addresses("linear_microscaled")
     if weight.bits != 4 or weight.width != x.width:
         raise KernelError(f"linear_microscaled: a weight of {weight.width} columns in {weight.bits} bits for rows of {x.width} (the widths must agree, weights have 4 bits)")
     code = dtype_code(out_dtype)
     if status is not None:
         _check(status, "status", torch.int32)
-    tokens, rows = x.codes.shape[0], weight.codes.shape[0]
-    out = torch.empty((tokens, rows), dtype=out_dtype, device=x.codes.device)
+        _check_here("linear_microscaled", status)
+    tokens, rows = x.rows, weight.rows
+    out = (x._store if x._store is not None else x._codes).new_empty((tokens, rows), dtype=out_dtype)
     if tokens and rows:
-        code = _lib().lb_gemm_microscaled(x.codes, x.scales, weight.codes, weight.scales, out, tokens, rows, chunks, x.bits, 1 if code == 0 else 0, status, _stream())
+        code = _lib().lb_gemm_microscaled(codes, scales, weight_codes, weight_scales, out, tokens, rows, x.chunks, x.bits, 1 if code == 0 else 0, status, _stream())
         if code == -5:
             raise KernelError("linear_microscaled: the driver gave no tensor map (cuTensorMapEncodeTiled)")
         _done(code, "gemm_microscaled")
@@ -2692,22 +2718,24 @@ def linear_microscaled(x: Microscaled, weight: Microscaled, out_dtype: torch.dty
 def gated_linear_microscaled(x: Microscaled, up: Microscaled, gate: Microscaled, activation: str, limit: float = 0.0, status: torch.Tensor | None = None) -> Microscaled:
     """``(x @ up.T) * act(x @ gate.T)`` of microscaled rows (8 or 4 bits) and weights (4 bits, ``[hidden, width]`` each), in 8 bits: sums, activation and product
     in 32 bits, then :func:`microscale`'s rule.  ``limit``: of the ``"sigmoid_limit"`` activation.  ``status`` as in :func:`linear_microscaled`."""
-    chunks = _check_microscaled(x, "gated_linear_microscaled")
-    _check_microscaled(up, "gated_linear_microscaled")
-    _check_microscaled(gate, "gated_linear_microscaled")
+    codes, scales = x._addresses("gated_linear_microscaled")
+    up_codes, up_scales = up._addresses("gated_linear_microscaled")
+    gate_codes, gate_scales = gate._addresses("gated_linear_microscaled")
     if activation not in _ACTIVATIONS:
         raise KernelError(f"unknown activation {activation!r}; known: {sorted(_ACTIVATIONS)}")
-    if up.bits != 4 or gate.bits != 4 or up.width != x.width or up.shape != gate.shape:
+    if up.bits != 4 or gate.bits != 4 or not up.width == gate.width == x.width or up.rows != gate.rows:
         raise KernelError(f"gated_linear_microscaled: weights of {tuple(up.shape)} in {up.bits} bits and {tuple(gate.shape)} in {gate.bits} for rows of {x.width} "
                           "(both must be [hidden, width] in 4 bits)")
     if status is not None:
         _check(status, "status", torch.int32)
-    tokens, hidden = x.codes.shape[0], up.codes.shape[0]
+        _check_here("gated_linear_microscaled", status)
+    tokens, hidden = x.rows, up.rows
     if not hidden:
         raise KernelError("gated_linear_microscaled: the weights have no rows")
-    out = Microscaled.empty(tokens, hidden, 8, x.codes.device)
+    out = Microscaled._empty(tokens, hidden, 8, x._store if x._store is not None else x._codes)
     if tokens:
-        code = _lib().lb_gated_microscaled(x.codes, x.scales, up.codes, up.scales, gate.codes, gate.scales, out.codes, out.scales, tokens, hidden, chunks, x.bits,
+        out_codes, out_scales = out._addresses("gated_linear_microscaled")
+        code = _lib().lb_gated_microscaled(codes, scales, up_codes, up_scales, gate_codes, gate_scales, out_codes, out_scales, tokens, hidden, x.chunks, x.bits,
                                            _ACTIVATIONS[activation], limit, status, _stream())
         if code == -5:
             raise KernelError("gated_linear_microscaled: the driver gave no tensor map (cuTensorMapEncodeTiled)")

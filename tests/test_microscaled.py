@@ -89,13 +89,22 @@ def test_the_stand_ins_reach_the_launch():
     ids=str,
 )
 def test_rows_that_are_none(bad):
-    broken = rows(3, 200, 8, bad)
+    with pytest.raises(ops.KernelError):
+        rows(3, 200, 8, bad)
+
+
+def test_rows_on_another_device(monkeypatch):
+    one, weight = rows(3, 200, 8), rows(5, 200, 4)
+    elsewhere = ops.Microscaled(on_cuda(aligned(5, 128), device=1), on_cuda(aligned(1, 2, 512), device=1), 200, 4)
     for call in (
-        lambda: broken.values(),
-        lambda: ops.linear_microscaled(broken, rows(5, 200, 4)),
-        lambda: ops.gated_linear_microscaled(broken, rows(5, 200, 4), rows(5, 200, 4), "silu"),
+        lambda: ops.linear_microscaled(one, elsewhere),
+        lambda: ops.linear_microscaled(elsewhere, weight),
+        lambda: ops.gated_linear_microscaled(one, weight, elsewhere, "silu"),
+        lambda: ops.gated_linear_microscaled(one, elsewhere, weight, "silu"),
+        lambda: ops.linear_microscaled(one, weight, status=on_cuda(torch.zeros(1, dtype=torch.int32), device=1)),
+        lambda: elsewhere.values(),
     ):
-        with pytest.raises(ops.KernelError):
+        with pytest.raises(ops.KernelError, match="device"):
             call()
 
 
