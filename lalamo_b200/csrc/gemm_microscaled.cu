@@ -38,6 +38,21 @@ __device__ __forceinline__ void bulk_load(void* destination, const void* source,
                  : "memory");
 }
 
+// True in one lane of the warp.  The copying and the issuing warp walk their loops as a whole, and one lane, elected each time, issues: inside a branch on the
+// lane's number the same instructions took 55 cycles each, which bounded a stage of the ring at 500.
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t elected;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(elected));
+    return elected != 0u;
+}
+
+// A whole warp waits, and its lanes go on together or not at all.  (Where one lane waited for the others, what the warp issues afterwards took twice as long.)
+__device__ __forceinline__ bool barrier_wait_warp(uint64_t* barrier, uint32_t parity) { return __all_sync(0xffffffffu, barrier_wait_parked(barrier, parity)); }
+
 // A tile of scales, 32 rows of 16 bytes one behind the other (groups of 8 rows 128 bytes apart, no swizzle), for tcgen05.cp.
 __device__ __forceinline__ uint64_t scale_descriptor(const void* tile) {
     const uint64_t address = smem_address(tile);
@@ -111,14 +126,43 @@ struct MsShape {
     static constexpr uint32_t kWCounted = BITS == 8 ? kWBytes / 2 : kWBytes;
 };
 
-constexpr int kMsThreads = 12 * 32;             // producer, issuer, scales of a gated product, one idle; eight warps of the epilogue
-constexpr int kMsRegionBytes = 20 * 1024;       // per half of the epilogue: two output buffers of 8 KB; gated: two of 2 KB and four handovers of 4 KB
+// One lane's work on a stage that has landed, of `chunks` 128s: its scales to tensor memory, its four products, and the stage's return to the producer.
+template <int BITS, int BN>
+__device__ __forceinline__ void issue_stage(uint32_t tmem_d, const unsigned char* stage, uint32_t columns, uint32_t token_column, uint32_t idesc, int chunks, bool accumulate,
+                                            uint64_t* empty) {
+    using Shape = MsShape<BITS, BN>;
+    const unsigned char* scales = stage + Shape::kWBytes + Shape::kXBytes;
+#pragma unroll
+    for (int c = 0; c < Shape::kChunks; ++c) {
+        if (c >= chunks) break;
+        copy_scales(columns + 4 * c, scales + c * kScaleTileBytes);
+#pragma unroll
+        for (int t = 0; t < Shape::kScaleTiles; ++t)
+            copy_scales(columns + 4 * (Shape::kChunks + c * Shape::kScaleTiles + t), scales + Shape::kWScaleBytes + (t * Shape::kChunks + c) * kScaleTileBytes);
+    }
+    const uint64_t desc_w = tile_descriptor(stage), desc_x = tile_descriptor(stage + Shape::kWBytes);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int c = product_chunk<BITS>(k);
+        if (c >= chunks) break;
+        mma_microscaled<BITS>(tmem_d, desc_w + 2 * k, desc_x + 2 * k, idesc | product_scales<BITS>(k), columns + 4 * c,
+                              columns + 4 * (Shape::kChunks + c * Shape::kScaleTiles) + token_column, accumulate || k > 0);
+    }
+    mma_commit(empty);
+}
+
+constexpr int kMsThreads = 20 * 32;             // producer, issuer, scales of a gated product, one idle; sixteen warps of the epilogue
+constexpr int kMsGroup = 16;                    // tokens that four warps of the epilogue take at a time
+constexpr int kMsTurnedPitch = kMsRows + 4;     // floats: the 16 bytes of eight lanes and of the next token's lie in different banks
+constexpr int kMsTurnedBytes = kMsGroup * kMsTurnedPitch * 4;
+constexpr int kMsRegionBytes = 11 * 1024;       // per four warps: gated, 16 tokens turned over and two output buffers; else two output buffers of bfloat16, or one of float32
+static_assert(kMsRegionBytes >= kMsTurnedBytes + 2 * kMsGroup * 64 && kMsRegionBytes >= kMsGroup * kMsRows * 4, "room for either");
 constexpr int kMsSharedLimit = 227 * 1024;
 
 template <int BITS, int BN>
 struct MsWalk {
-    static constexpr int kStages = (kMsSharedLimit - 2 * kMsRegionBytes - 1024 - 256) / MsShape<BITS, BN>::kStageBytes;
-    static constexpr int kBytes = kStages * MsShape<BITS, BN>::kStageBytes + 2 * kMsRegionBytes + 1024 + 256;
+    static constexpr int kStages = (kMsSharedLimit - 4 * kMsRegionBytes - 1024 - 256) / MsShape<BITS, BN>::kStageBytes;
+    static constexpr int kBytes = kStages * MsShape<BITS, BN>::kStageBytes + 4 * kMsRegionBytes + 1024 + 256;
     static constexpr int kScaleColumns = 4 * MsShape<BITS, BN>::kChunks * (1 + MsShape<BITS, BN>::kScaleTiles);
     static constexpr int kColumns = 2 * BN + kScaleColumns <= 256 ? 256 : 512;
     static_assert(kStages >= 3 && kStages <= 12 && 2 * BN + kScaleColumns <= 512, "a ring, its barriers, two accumulators and the scales");
@@ -136,7 +180,7 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     extern __shared__ unsigned char raw_shared[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_shared) + 1023) & ~static_cast<uintptr_t>(1023));
     unsigned char* regions = ring + STAGES * Shape::kStageBytes;
-    uint64_t* barriers = reinterpret_cast<uint64_t*>(regions + 2 * kMsRegionBytes);
+    uint64_t* barriers = reinterpret_cast<uint64_t*>(regions + 4 * kMsRegionBytes);
     uint64_t* full = barriers;
     uint64_t* empty = barriers + STAGES;
     uint64_t* tmem_full = barriers + 2 * STAGES;
@@ -144,7 +188,7 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(barriers + 2 * STAGES + 4);
     __shared__ int failed;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     constexpr int kRowsPerTile = GATED ? kMsRows / 2 : kMsRows;
     const int num_stages = (p.chunks + Shape::kChunks - 1) / Shape::kChunks;
     const int num_tiles = p.row_tiles * p.token_tiles;
@@ -157,7 +201,7 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         }
         for (int a = 0; a < 2; ++a) {
             barrier_init(&tmem_full[a], 1);
-            barrier_init(&tmem_empty[a], 8);
+            barrier_init(&tmem_empty[a], 16);
         }
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -170,85 +214,61 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
-    const uint32_t tmem_w_scales = tmem_base + 2 * BN, tmem_x_scales = tmem_w_scales + 4 * Shape::kChunks;
+    const uint32_t tmem_scales = tmem_base + 2 * BN;
     // Everything that is read may come from the kernel before this one, the weights too (quantised just now).
     wait_for_previous_kernel();
     allow_next_kernel();
 
-    if (warp == 0 && lane == 0) {
-        int issued = 0;
+    if (warp == 0) {
+        int s = 0, round = 0;
         bool ok = true;
         for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
             const int row0 = (tile % p.row_tiles) * kRowsPerTile, token0 = (tile / p.row_tiles) * BN;
             const int scale_tiles = min(Shape::kScaleTiles, (p.tokens + 127) / 128 - token0 / 128);
             const unsigned char* w_scales = p.w_scales + static_cast<size_t>(row0 / 128) * p.chunks * kScaleTileBytes;
             const unsigned char* x_scales = p.x_scales + static_cast<size_t>(token0 / 128) * p.chunks * kScaleTileBytes;
-            for (int stage = 0; stage < num_stages; ++stage, ++issued) {
-                const int s = issued % STAGES, round = issued / STAGES;
-                if (round > 0 && !barrier_wait(&empty[s], (round - 1) & 1)) {
+            for (int stage = 0; stage < num_stages; ++stage) {
+                ok = round == 0 || barrier_wait_warp(&empty[s], (round - 1) & 1);
+                if (!ok) {
                     atomicExch(&failed, 1);
-                    ok = false;
                     break;
                 }
-                unsigned char* at = ring + s * Shape::kStageBytes;
-                const int column = stage * 128;   // of the map: elements of W where they are spread and of X in 8 bits, bytes of rows in 4
-                const int chunk = stage * Shape::kChunks;
-                const uint32_t scale_bytes = static_cast<uint32_t>(chunks_of(stage) * kScaleTileBytes);
-                barrier_expect(&full[s], Shape::kWCounted + Shape::kXBytes + (GATED ? 0u : scale_bytes) + scale_tiles * scale_bytes);
-                tma_load_2d(at, &map_w, column, row0, &full[s]);
-                if constexpr (GATED) tma_load_2d(at + Shape::kWBytes / 2, &map_gate, column, row0, &full[s]);
-                tma_load_2d(at + Shape::kWBytes, &map_x, column, token0, &full[s]);
-                at += Shape::kWBytes + Shape::kXBytes;
-                if constexpr (!GATED) bulk_load(at, w_scales + static_cast<size_t>(chunk) * kScaleTileBytes, scale_bytes, &full[s]);
-                at += Shape::kWScaleBytes;
-                for (int t = 0; t < scale_tiles; ++t)
-                    bulk_load(at + t * Shape::kWScaleBytes, x_scales + (static_cast<size_t>(t) * p.chunks + chunk) * kScaleTileBytes, scale_bytes, &full[s]);
+                if (elect_lane()) {
+                    unsigned char* at = ring + s * Shape::kStageBytes;
+                    const int column = stage * 128;   // of the map: elements of W where they are spread and of X in 8 bits, bytes of rows in 4
+                    const int chunk = stage * Shape::kChunks;
+                    const uint32_t scale_bytes = static_cast<uint32_t>(chunks_of(stage) * kScaleTileBytes);
+                    barrier_expect(&full[s], Shape::kWCounted + Shape::kXBytes + (GATED ? 0u : scale_bytes) + scale_tiles * scale_bytes);
+                    tma_load_2d(at, &map_w, column, row0, &full[s]);
+                    if constexpr (GATED) tma_load_2d(at + Shape::kWBytes / 2, &map_gate, column, row0, &full[s]);
+                    tma_load_2d(at + Shape::kWBytes, &map_x, column, token0, &full[s]);
+                    at += Shape::kWBytes + Shape::kXBytes;
+                    if constexpr (!GATED) bulk_load(at, w_scales + static_cast<size_t>(chunk) * kScaleTileBytes, scale_bytes, &full[s]);
+                    at += Shape::kWScaleBytes;
+                    for (int t = 0; t < scale_tiles; ++t)
+                        bulk_load(at + t * Shape::kWScaleBytes, x_scales + (static_cast<size_t>(t) * p.chunks + chunk) * kScaleTileBytes, scale_bytes, &full[s]);
+                }
+                if (++s == STAGES) s = 0, ++round;
             }
         }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
         const uint32_t idesc = microscaled_descriptor<BITS>(BN);
-        int consumed = 0, local = 0;
+        int s = 0, round = 0, local = 0;
         bool ok = true;
         for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++local) {
             const int accumulator = local & 1, use = local >> 1;
-            if (use > 0 && !barrier_wait(&tmem_empty[accumulator], (use - 1) & 1)) {
-                atomicExch(&failed, 1);
-                break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            ok = use == 0 || barrier_wait_warp(&tmem_empty[accumulator], (use - 1) & 1);
             const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(accumulator * BN);
-            const int token0 = (tile / p.row_tiles) * BN;
-            const uint32_t x_scales = tmem_x_scales + static_cast<uint32_t>((token0 & 127) >> 5);   // 32 tokens a column
-            for (int stage = 0; stage < num_stages; ++stage, ++consumed) {
-                const int s = consumed % STAGES, round = consumed / STAGES;
-                if (!barrier_wait(&full[s], round & 1)) {
-                    atomicExch(&failed, 1);
-                    ok = false;
-                    break;
-                }
+            const uint32_t token_column = static_cast<uint32_t>((((tile / p.row_tiles) * BN) & 127) >> 5);   // of the scales: 32 tokens a column
+            for (int stage = 0; stage < num_stages && ok; ++stage) {
+                ok = barrier_wait_warp(&full[s], round & 1);
+                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                unsigned char* at = ring + s * Shape::kStageBytes;
-                const unsigned char* scales = at + Shape::kWBytes + Shape::kXBytes;
-                const int here = chunks_of(stage);
-#pragma unroll
-                for (int c = 0; c < Shape::kChunks; ++c) {
-                    if (c >= here) break;
-                    copy_scales(tmem_w_scales + 4 * c, scales + c * kScaleTileBytes);
-#pragma unroll
-                    for (int t = 0; t < Shape::kScaleTiles; ++t)
-                        copy_scales(tmem_x_scales + 4 * (c * Shape::kScaleTiles + t), scales + Shape::kWScaleBytes + (t * Shape::kChunks + c) * kScaleTileBytes);
-                }
-                const uint64_t desc_w = tile_descriptor(at), desc_x = tile_descriptor(at + Shape::kWBytes);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int c = product_chunk<BITS>(k);
-                    if (c >= here) break;
-                    mma_microscaled<BITS>(tmem_d, desc_w + 2 * k, desc_x + 2 * k, idesc | product_scales<BITS>(k), tmem_w_scales + 4 * c,
-                                          x_scales + 4 * Shape::kScaleTiles * c, stage > 0 || k > 0);
-                }
-                mma_commit(&empty[s]);
+                if (elect_lane()) issue_stage<BITS, BN>(tmem_d, ring + s * Shape::kStageBytes, tmem_scales, token_column, idesc, chunks_of(stage), stage > 0, &empty[s]);
+                if (++s == STAGES) s = 0, ++round;
             }
-            if (ok) mma_commit(&tmem_full[accumulator]);
+            if (!ok) atomicExch(&failed, 1);
+            else if (elect_lane()) mma_commit(&tmem_full[accumulator]);
         }
     } else if (GATED && warp == 2) {
         // Lane l puts together the 16 bytes of the rows l, l + 32 of `up` and of `gate` in the accumulator's order.  Four stages are read at once: a
@@ -276,8 +296,7 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                 for (int i = 0; i < 4; ++i) {
                     if (first + i >= num_stages) break;
                     const int s = issued % STAGES, round = issued / STAGES;
-                    // the lanes go on together or not at all
-                    ok = __all_sync(0xffffffffu, round == 0 || barrier_wait(&empty[s], (round - 1) & 1));
+                    ok = round == 0 || barrier_wait_warp(&empty[s], (round - 1) & 1);
                     if (!ok) {
                         atomicExch(&failed, 1);
                         break;
@@ -294,18 +313,15 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
             }
         }
     } else if (warp >= 4) {
-        // Eight warps: warp & 3 is the quarter of the lanes that a warp may read, and each half of the tokens has four warps.
-        const int quarter = warp & 3, half = (warp - 4) >> 2;
-        constexpr int kLowerPart = (BN / 2 + 31) / 32 * 32;   // whole 32s
-        const int part_begin = half ? kLowerPart : 0, part_tokens = half ? BN - kLowerPart : kLowerPart;
-        const int half_barrier = 5 + half;   // 1 to 4 belong to the pairs of warps of the gated epilogue
+        // Sixteen warps in four sets: warp & 3 is the quarter of the lanes that a warp may read, and the sets take 16 tokens at a time in turn.
+        const int quarter = warp & 3, set = (warp - 4) >> 2, set_barrier = 1 + set;
         const bool issuer = quarter == 0 && lane == 0;
-        unsigned char* region = regions + half * kMsRegionBytes;
+        unsigned char* region = regions + set * kMsRegionBytes;
         int local = 0, groups = 0;
         for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++local) {
             const int accumulator = local & 1, use = local >> 1;
-            const int row0 = (tile % p.row_tiles) * kRowsPerTile, token0 = (tile / p.row_tiles) * BN + part_begin;
-            uint32_t arrived = barrier_wait(&tmem_full[accumulator], use & 1) ? 1u : 0u;
+            const int row0 = (tile % p.row_tiles) * kRowsPerTile, token0 = (tile / p.row_tiles) * BN;
+            uint32_t arrived = barrier_wait_warp(&tmem_full[accumulator], use & 1) ? 1u : 0u;
             {
                 // Warps that meet at named barriers below go on together or not at all.
                 uint32_t all;
@@ -317,7 +333,7 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                     "selp.u32 %0, 1, 0, all;\n"
                     "}\n"
                     : "=r"(all)
-                    : "r"(arrived), "r"(half_barrier)
+                    : "r"(arrived), "r"(set_barrier)
                     : "memory");
                 arrived = all;
             }
@@ -326,72 +342,81 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(accumulator * BN + part_begin) + (static_cast<uint32_t>(quarter * 32) << 16);
-            const int step = !GATED && p.out_is_float && p.bulk_store ? 16 : 32;
+            const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(accumulator * BN) + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-            for (int column = 0; column < part_tokens; column += step, ++groups) {
-                if (token0 + column >= p.tokens) break;   // the same for the whole half
+            for (int column = set * kMsGroup; column < BN; column += 4 * kMsGroup, ++groups) {
+                const int first_token = token0 + column;
+                if (first_token >= p.tokens) break;   // the same for the whole set
+                uint32_t v[kMsGroup];
+                tmem_load_16(tmem_d + static_cast<uint32_t>(column), v);
                 if constexpr (GATED) {
-                    unsigned char* out_buffer = region + (groups & 1) * 2048;
+                    // Lanes 0 to 63 hold `up` and lanes 64 to 127 the same rows of `gate`: turned over in shared memory, so that a thread has eight
+                    // channels of a token (four of every 32) and eight threads its 64.
+                    float* turned = reinterpret_cast<float*>(region);
+                    unsigned char* out_buffer = region + kMsTurnedBytes + (groups & 1) * (kMsGroup * 64);
+#pragma unroll
+                    for (int i = 0; i < kMsGroup; ++i) turned[i * kMsTurnedPitch + quarter * 32 + lane] = __uint_as_float(v[i]);
                     if (issuer) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // the store before last has read this buffer
-                    named_barrier(half_barrier, 128);
-                    uint32_t v[32];
-                    tmem_load_32(tmem_d + static_cast<uint32_t>(column), v);
-                    // Lanes 64 to 127 hold `gate`, lanes 0 to 63 the same rows of `up`: handed over in 32 bits.
-                    float* handover = reinterpret_cast<float*>(region + 4096 + ((quarter & 1) * 2 + (groups & 1)) * 4096) + lane;
-                    const int pair_barrier = 1 + half * 2 + (quarter & 1);
-                    if (quarter >= 2) {
+                    named_barrier(set_barrier, 128);
+                    const int token_here = quarter * 4 + (lane >> 3), part = lane & 7;
+                    float h[2][4];
+                    int byte[2];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) handover[i * 32] = ms_gate_side(__uint_as_float(v[i]), p.activation, p.limit);
-                        named_barrier(pair_barrier, 64);
-                    } else {
-                        named_barrier(pair_barrier, 64);
-                        const bool exists = row0 + quarter * 32 + lane < p.n;   // past the last row: zeros, whatever the scales there
-                        int kept = 0;
+                    for (int b = 0; b < 2; ++b) {
+                        const float* from = turned + token_here * kMsTurnedPitch + b * 32 + part * 4;
+                        const float4 u = *reinterpret_cast<const float4*>(from), g = *reinterpret_cast<const float4*>(from + kMsRows / 2);
+                        h[b][0] = ms_up_side(u.x, p.activation, p.limit) * ms_gate_side(g.x, p.activation, p.limit);
+                        h[b][1] = ms_up_side(u.y, p.activation, p.limit) * ms_gate_side(g.y, p.activation, p.limit);
+                        h[b][2] = ms_up_side(u.z, p.activation, p.limit) * ms_gate_side(g.z, p.activation, p.limit);
+                        h[b][3] = ms_up_side(u.w, p.activation, p.limit) * ms_gate_side(g.w, p.activation, p.limit);
+                        if (row0 + kMsRows / 2 > p.n) {   // past the last row: zeros, whatever the scales there
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            // A token's 32 lanes of this warp are one block of the output.
-                            const float h = exists ? ms_up_side(__uint_as_float(v[i]), p.activation, p.limit) * handover[i * 32] : 0.0f;
-                            const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
-                            const int byte = scale_byte<8>(largest);
-                            const float scaled = byte == kNoNumber ? 0.0f : h * scale_inverse(byte);
-                            out_buffer[i * 64 + quarter * 32 + lane] = static_cast<unsigned char>(pack_e4m3(scaled, 0.0f, 0.0f, 0.0f));
-                            if (lane == i) kept = byte;
+                            for (int i = 0; i < 4; ++i)
+                                if (row0 + b * 32 + part * 4 + i >= p.n) h[b][i] = 0.0f;
                         }
-                        const int token = token0 + column + lane, block = row0 / 32 + quarter;
-                        if (token < p.tokens) p.out_scales[scale_word(token, block >> 2, p.out_chunks) + (block & 3)] = static_cast<unsigned char>(kept);
                     }
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        float largest = larger_size(larger_size(h[b][0], h[b][1]), larger_size(h[b][2], h[b][3]));
+#pragma unroll
+                        for (int offset = 1; offset < 8; offset <<= 1) largest = larger_size(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
+                        byte[b] = scale_byte<8>(__float_as_uint(largest) & 0x7fffffffu);
+                        const float inverse = scale_inverse(byte[b]);
+                        *reinterpret_cast<uint32_t*>(out_buffer + token_here * 64 + b * 32 + part * 4) =
+                            pack_e4m3(h[b][0] * inverse, h[b][1] * inverse, h[b][2] * inverse, h[b][3] * inverse);
+                    }
+                    const int token = first_token + token_here, block = row0 / 32;   // an even one
+                    if (part == 0 && token < p.tokens)
+                        *reinterpret_cast<uint16_t*>(p.out_scales + scale_word(token, block >> 2, p.out_chunks) + (block & 3)) = static_cast<uint16_t>(byte[0] | byte[1] << 8);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    named_barrier(half_barrier, 128);
-                    if (issuer) bulk_store_2d(&map_out, out_buffer, row0, token0 + column, false);
+                    named_barrier(set_barrier, 128);
+                    if (issuer) bulk_store_2d(&map_out, out_buffer, row0, first_token, false);
                 } else if (p.bulk_store) {
-                    unsigned char* out_buffer = region + (groups & 1) * 8192;
-                    if (issuer) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-                    named_barrier(half_barrier, 128);
+                    // Stores issued by the threads themselves queue behind the loads of the stages.  One buffer of float32, or two of bfloat16.
+                    unsigned char* out_buffer = region + (p.out_is_float ? 0 : (groups & 1) * (kMsGroup * kMsRows * 2));
+                    if (issuer) {
+                        if (p.out_is_float) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    }
+                    named_barrier(set_barrier, 128);
                     if (p.out_is_float) {
-                        uint32_t v[16];
-                        tmem_load_16(tmem_d + static_cast<uint32_t>(column), v);
-                        float* stage = reinterpret_cast<float*>(out_buffer) + quarter * 32 + lane;
+                        float* to = reinterpret_cast<float*>(out_buffer) + quarter * 32 + lane;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) stage[i * kMsRows] = __uint_as_float(v[i]);
+                        for (int i = 0; i < kMsGroup; ++i) to[i * kMsRows] = __uint_as_float(v[i]);
                     } else {
-                        uint32_t v[32];
-                        tmem_load_32(tmem_d + static_cast<uint32_t>(column), v);
-                        __nv_bfloat16* stage = reinterpret_cast<__nv_bfloat16*>(out_buffer) + quarter * 32 + lane;
+                        __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(out_buffer) + quarter * 32 + lane;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) stage[i * kMsRows] = __float2bfloat16_rn(__uint_as_float(v[i]));
+                        for (int i = 0; i < kMsGroup; ++i) to[i * kMsRows] = __float2bfloat16_rn(__uint_as_float(v[i]));
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    named_barrier(half_barrier, 128);
-                    if (issuer) bulk_store_2d(&map_out, out_buffer, row0, token0 + column, false);
+                    named_barrier(set_barrier, 128);
+                    if (issuer) bulk_store_2d(&map_out, out_buffer, row0, first_token, false);
                 } else {
-                    uint32_t v[32];
-                    tmem_load_32(tmem_d + static_cast<uint32_t>(column), v);
-                    const int row = row0 + quarter * 32 + lane, tokens_here = min(32, p.tokens - token0 - column);
+                    const int row = row0 + quarter * 32 + lane, tokens_here = min(kMsGroup, p.tokens - first_token);
                     if (row < p.n) {
-                        const size_t first = static_cast<size_t>(token0 + column) * p.n + row;
+                        const size_t first = static_cast<size_t>(first_token) * p.n + row;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
+                        for (int i = 0; i < kMsGroup; ++i) {
                             if (i >= tokens_here) break;
                             if (p.out_is_float) static_cast<float*>(p.out)[first + static_cast<size_t>(i) * p.n] = __uint_as_float(v[i]);
                             else static_cast<__nv_bfloat16*>(p.out)[first + static_cast<size_t>(i) * p.n] = __float2bfloat16_rn(__uint_as_float(v[i]));
@@ -423,12 +448,12 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 // ---------------------------------------------------------------------------------------------
 constexpr int kMsSplitThreads = 256;   // producer, issuer, scales of a gated product, one idle, four that read tensor memory; all of them add up
 constexpr int kMsLargestSplit = 8;     // CTAs of a cluster
-constexpr int kMsSplitStages = 11;     // of the ring, at most
-constexpr int kMsSplitShared = kMsSharedLimit - 1024;   // beside the variables
+constexpr int kMsSplitStages = 8;      // of the ring, at most
+constexpr int kMsSplitShared = 112 * 1024;   // beside the variables: half a multiprocessor's
 
 template <int BITS, int BN>
 struct MsSplit {
-    static constexpr int kScaleColumns = 4 * MsShape<BITS, BN>::kChunks * 2;
+    static constexpr int kScaleColumns = 4 * MsShape<BITS, BN>::kChunks * (1 + MsShape<BITS, BN>::kScaleTiles);
     static constexpr int kColumns = BN + kScaleColumns <= 32 ? 32 : BN + kScaleColumns <= 64 ? 64 : BN + kScaleColumns <= 128 ? 128 : 256;
     static constexpr int kPartBytes = BN * kMsRows * 4;   // the parts' sums, where the ring was
     static constexpr int kSlack = 1024 + 256;             // alignment and barriers
@@ -440,10 +465,10 @@ struct MsSplit {
     }
 };
 
-__device__ __forceinline__ float load_cluster(uint32_t address) {
-    float value;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(value) : "r"(address) : "memory");
-    return value;
+__device__ __forceinline__ float4 load_cluster(uint32_t address) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address));
+    return v;
 }
 
 template <int BITS, int BN, bool GATED>
@@ -462,7 +487,7 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
     uint64_t* empty = barriers + kMsSplitStages;
     uint64_t* accumulated = barriers + 2 * kMsSplitStages;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     constexpr int kRowsPerTile = GATED ? kMsRows / 2 : kMsRows;
     const int rank = static_cast<int>(blockIdx.x) % splits;   // the cluster's CTAs are neighbours
     const int row0 = static_cast<int>(blockIdx.x) / splits * kRowsPerTile, token0 = blockIdx.y * BN;
@@ -487,61 +512,44 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = tmem_slot;
-    const uint32_t tmem_w_scales = tmem_base + BN, tmem_x_scales = tmem_w_scales + 4 * Shape::kChunks;
     wait_for_previous_kernel();   // the weights may be what it has made
     allow_next_kernel();
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
         const unsigned char* w_scales = p.w_scales + static_cast<size_t>(row0 / 128) * p.chunks * kScaleTileBytes;
         const unsigned char* x_scales = p.x_scales + static_cast<size_t>(token0 / 128) * p.chunks * kScaleTileBytes;
         for (int i = 0, s = 0, round = 0; i < count; ++i) {
-            if (round > 0 && !barrier_wait(&empty[s], (round - 1) & 1)) {
+            if (round > 0 && !barrier_wait_warp(&empty[s], (round - 1) & 1)) {
                 atomicExch(&failed, 1);
                 break;
             }
-            const int stage = first_stage + i, column = stage * 128, chunk = stage * Shape::kChunks;
-            unsigned char* at = ring + s * Shape::kStageBytes;
-            const uint32_t scale_bytes = static_cast<uint32_t>(chunks_of(stage) * kScaleTileBytes);
-            barrier_expect(&full[s], Shape::kWCounted + Shape::kXBytes + (GATED ? 1u : 2u) * scale_bytes);
-            tma_load_2d(at, &map_w, column, row0, &full[s]);
-            if constexpr (GATED) tma_load_2d(at + Shape::kWBytes / 2, &map_gate, column, row0, &full[s]);
-            tma_load_2d(at + Shape::kWBytes, &map_x, column, token0, &full[s]);
-            at += Shape::kWBytes + Shape::kXBytes;
-            if constexpr (!GATED) bulk_load(at, w_scales + static_cast<size_t>(chunk) * kScaleTileBytes, scale_bytes, &full[s]);
-            bulk_load(at + Shape::kWScaleBytes, x_scales + static_cast<size_t>(chunk) * kScaleTileBytes, scale_bytes, &full[s]);
+            if (elect_lane()) {
+                const int stage = first_stage + i, column = stage * 128, chunk = stage * Shape::kChunks;
+                unsigned char* at = ring + s * Shape::kStageBytes;
+                const uint32_t scale_bytes = static_cast<uint32_t>(chunks_of(stage) * kScaleTileBytes);
+                barrier_expect(&full[s], Shape::kWCounted + Shape::kXBytes + (GATED ? 1u : 2u) * scale_bytes);
+                tma_load_2d(at, &map_w, column, row0, &full[s]);
+                if constexpr (GATED) tma_load_2d(at + Shape::kWBytes / 2, &map_gate, column, row0, &full[s]);
+                tma_load_2d(at + Shape::kWBytes, &map_x, column, token0, &full[s]);
+                at += Shape::kWBytes + Shape::kXBytes;
+                if constexpr (!GATED) bulk_load(at, w_scales + static_cast<size_t>(chunk) * kScaleTileBytes, scale_bytes, &full[s]);
+                bulk_load(at + Shape::kWScaleBytes, x_scales + static_cast<size_t>(chunk) * kScaleTileBytes, scale_bytes, &full[s]);
+            }
             if (++s == ring_stages) s = 0, ++round;
         }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
         const uint32_t idesc = microscaled_descriptor<BITS>(BN);
-        const uint32_t x_column = tmem_x_scales + static_cast<uint32_t>((token0 & 127) >> 5);
         bool ok = true;
         for (int i = 0, s = 0, round = 0; i < count; ++i) {
-            if (!barrier_wait(&full[s], round & 1)) {
-                atomicExch(&failed, 1);
-                ok = false;
-                break;
-            }
+            ok = barrier_wait_warp(&full[s], round & 1);
+            if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            unsigned char* at = ring + s * Shape::kStageBytes;
-            const unsigned char* scales = at + Shape::kWBytes + Shape::kXBytes;
-            const int here = chunks_of(first_stage + i);
-#pragma unroll
-            for (int c = 0; c < Shape::kChunks; ++c) {
-                if (c >= here) break;
-                copy_scales(tmem_w_scales + 4 * c, scales + c * kScaleTileBytes);
-                copy_scales(tmem_x_scales + 4 * c, scales + Shape::kWScaleBytes + c * kScaleTileBytes);
-            }
-            const uint64_t desc_w = tile_descriptor(at), desc_x = tile_descriptor(at + Shape::kWBytes);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int c = product_chunk<BITS>(k);
-                if (c >= here) break;
-                mma_microscaled<BITS>(tmem_base, desc_w + 2 * k, desc_x + 2 * k, idesc | product_scales<BITS>(k), tmem_w_scales + 4 * c, x_column + 4 * c, i > 0 || k > 0);
-            }
-            mma_commit(&empty[s]);
+            if (elect_lane())
+                issue_stage<BITS, BN>(tmem_base, ring + s * Shape::kStageBytes, tmem_base + BN, static_cast<uint32_t>((token0 & 127) >> 5), idesc, chunks_of(first_stage + i), i > 0, &empty[s]);
             if (++s == ring_stages) s = 0, ++round;
         }
-        if (ok) mma_commit(accumulated);
+        if (!ok) atomicExch(&failed, 1);
+        else if (elect_lane()) mma_commit(accumulated);
     } else if (GATED && warp == 2) {
         // as in the walking kernel
         const size_t offset = static_cast<size_t>(row0 / 128) * p.chunks * kScaleTileBytes + lane * 16 + ((row0 & 64) >> 3);
@@ -563,7 +571,7 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (first + i >= count) break;
-                ok = __all_sync(0xffffffffu, round == 0 || barrier_wait(&empty[s], (round - 1) & 1));
+                ok = round == 0 || barrier_wait_warp(&empty[s], (round - 1) & 1);
                 if (!ok) {
                     atomicExch(&failed, 1);
                     break;
@@ -579,8 +587,7 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
         }
     } else if (warp >= 4) {
         const int quarter = warp & 3;
-        const bool ok = __all_sync(0xffffffffu, barrier_wait(accumulated, 0));
-        if (ok) {
+        if (barrier_wait_warp(accumulated, 0)) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float* part = reinterpret_cast<float*>(ring) + quarter * 32 + lane;
 #pragma unroll 1
@@ -600,44 +607,85 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
     cluster_sync();   // all parts are there, or some CTA has failed and says so below
     const int tokens_here = min(BN, p.tokens - token0);
     const uint32_t part = smem_address(ring);
-    uint32_t parts[kMsLargestSplit];
+    // Four rows (of a token) at each of two places, part after part; all parts are read before the first is added.
+    auto add_up = [&](int first, int second, float4 (&sums)[2]) {
+        float4 v[kMsLargestSplit], w[kMsLargestSplit];
 #pragma unroll
-    for (int q = 0; q < kMsLargestSplit; ++q) {
-        parts[q] = part;
-        if (q < splits) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(parts[q]) : "r"(part), "r"(q));
-    }
-    auto sum_of = [&](int token, int row) {
-        const uint32_t offset = static_cast<uint32_t>(token * kMsRows + row) * 4u;
-        float v[kMsLargestSplit], sum = 0.0f;
+        for (int q = 0; q < kMsLargestSplit; ++q) {
+            if (q < splits) {
+                uint32_t at;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(part), "r"(q));
+                v[q] = load_cluster(at + first * 4);
+                w[q] = load_cluster(at + second * 4);
+            }
+        }
+        sums[0] = v[0], sums[1] = w[0];
 #pragma unroll
-        for (int q = 0; q < kMsLargestSplit; ++q) v[q] = q < splits ? load_cluster(parts[q] + offset) : 0.0f;
-#pragma unroll
-        for (int q = 0; q < kMsLargestSplit; ++q) sum = q == 0 ? v[0] : q < splits ? sum + v[q] : sum;
-        return sum;
+        for (int q = 1; q < kMsLargestSplit; ++q) {
+            if (q < splits) {
+                sums[0].x += v[q].x, sums[0].y += v[q].y, sums[0].z += v[q].z, sums[0].w += v[q].w;
+                sums[1].x += w[q].x, sums[1].y += w[q].y, sums[1].z += w[q].z, sums[1].w += w[q].w;
+            }
+        }
     };
     if constexpr (!GATED) {
-        const int row = threadIdx.x & 127;
-        if (row0 + row < p.n) {
-#pragma unroll 2
-            for (int t = rank + (threadIdx.x >> 7) * splits; t < tokens_here; t += 2 * splits) {
-                const float sum = sum_of(t, row);
-                const size_t at = static_cast<size_t>(token0 + t) * p.n + row0 + row;
-                if (p.out_is_float) static_cast<float*>(p.out)[at] = sum;
-                else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(sum);
+        // A warp takes two tokens at a time, a lane four rows of each.
+        const int row = row0 + lane * 4;
+        for (int t = rank + 2 * warp * splits; t < tokens_here; t += 16 * splits) {
+            float4 sums[2];
+            add_up(t * kMsRows + lane * 4, (t + splits < tokens_here ? t + splits : t) * kMsRows + lane * 4, sums);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int token = t + i * splits;
+                if (token >= tokens_here) break;
+                const size_t at = static_cast<size_t>(token0 + token) * p.n + row;
+                if (p.bulk_store && row < p.n) {   // four rows are 16 (8) aligned bytes
+                    if (p.out_is_float) {
+                        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = sums[i];
+                    } else {
+                        uint2 packed;
+                        __nv_bfloat162* halves = reinterpret_cast<__nv_bfloat162*>(&packed);
+                        halves[0] = __floats2bfloat162_rn(sums[i].x, sums[i].y);
+                        halves[1] = __floats2bfloat162_rn(sums[i].z, sums[i].w);
+                        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) = packed;
+                    }
+                } else {
+                    const float values[4] = {sums[i].x, sums[i].y, sums[i].z, sums[i].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (row + e >= p.n) break;
+                        if (p.out_is_float) static_cast<float*>(p.out)[at + e] = values[e];
+                        else static_cast<__nv_bfloat16*>(p.out)[at + e] = __float2bfloat16_rn(values[e]);
+                    }
+                }
             }
         }
     } else {
-        // A warp takes a block of 32 channels of a token at a time.
-        const int half = warp & 1, channel = half * 32 + lane;
-        const bool exists = row0 + channel < p.n;
-        for (int t = rank + (warp >> 1) * splits; t < tokens_here; t += 4 * splits) {
-            const float u = sum_of(t, channel), g = sum_of(t, kMsRows / 2 + channel);
-            const float h = exists ? ms_up_side(u, p.activation, p.limit) * ms_gate_side(g, p.activation, p.limit) : 0.0f;
-            const int byte = scale_byte<8>(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu));
-            const float scaled = byte == kNoNumber ? 0.0f : h * scale_inverse(byte);
-            const int token = token0 + t, block = row0 / 32 + half;
-            static_cast<unsigned char*>(p.out)[static_cast<size_t>(token) * p.out_chunks * 128 + row0 + channel] = static_cast<unsigned char>(pack_e4m3(scaled, 0.0f, 0.0f, 0.0f));
-            if (lane == 0) p.out_scales[scale_word(token, block >> 2, p.out_chunks) + (block & 3)] = static_cast<unsigned char>(byte);
+        // Half a warp takes a token, eight lanes a block of 32 channels.
+        const int channel = (lane & 15) * 4;
+        for (int first = rank + 2 * warp * splits; first < tokens_here; first += 16 * splits) {   // the same for the whole warp
+            const int t = first + (lane >> 4) * splits;
+            const bool valid = t < tokens_here;
+            const int at = (valid ? t : first) * kMsRows + channel;
+            float4 sums[2];
+            add_up(at, at + kMsRows / 2, sums);
+            const float up[4] = {sums[0].x, sums[0].y, sums[0].z, sums[0].w}, gate[4] = {sums[1].x, sums[1].y, sums[1].z, sums[1].w};
+            float h[4], largest = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                h[e] = row0 + channel + e < p.n ? ms_up_side(up[e], p.activation, p.limit) * ms_gate_side(gate[e], p.activation, p.limit) : 0.0f;
+                largest = larger_size(largest, h[e]);
+            }
+#pragma unroll
+            for (int offset = 1; offset < 8; offset <<= 1) largest = larger_size(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
+            const int byte = scale_byte<8>(__float_as_uint(largest) & 0x7fffffffu);
+            const float inverse = scale_inverse(byte);
+            const int token = token0 + t, block = (row0 + channel) / 32;
+            if (valid) {
+                *reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.out) + static_cast<size_t>(token) * p.out_chunks * 128 + row0 + channel) =
+                    pack_e4m3(h[0] * inverse, h[1] * inverse, h[2] * inverse, h[3] * inverse);
+                if ((lane & 7) == 0) p.out_scales[scale_word(token, block >> 2, p.out_chunks) + (block & 3)] = static_cast<unsigned char>(byte);
+            }
         }
     }
     __syncthreads();
@@ -683,14 +731,14 @@ int launch_microscaled(const void* x, const void* w, const void* gate, MsParams 
     map_gate = map_w, map_out = map_x;
     if constexpr (GATED) {
         if (!make_codes_map(&map_gate, gate, p.n, w_bytes, kMsRows / 2, BITS == 8) ||
-            !make_ms_out_map(&map_out, p.out, p.tokens, p.out_chunks * 128, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, kMsRows / 2, 32))
+            !make_ms_out_map(&map_out, p.out, p.tokens, p.out_chunks * 128, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, kMsRows / 2, kMsGroup))
             return -5;
         p.row_tiles = p.out_chunks * 2;
     } else {
         const int size = p.out_is_float ? 4 : 2;
         p.bulk_store = (static_cast<size_t>(p.n) * size) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 ? 1 : 0;
         if (p.bulk_store && !make_ms_out_map(&map_out, p.out, p.tokens, p.n, p.out_is_float ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, size,
-                                             kMsRows, p.out_is_float ? 16 : 32))
+                                             kMsRows, kMsGroup))
             return -5;
         p.row_tiles = (p.n + kMsRows - 1) / kMsRows;
     }
@@ -709,13 +757,15 @@ int launch_microscaled_split(const void* x, const void* w, const void* gate, MsP
     if (!make_codes_map(&map_w, w, p.n, w_bytes, GATED ? kMsRows / 2 : kMsRows, BITS == 8) || !make_codes_map(&map_x, x, p.tokens, x_bytes, BN, false)) return -5;
     map_gate = map_w;
     if (GATED && !make_codes_map(&map_gate, gate, p.n, w_bytes, kMsRows / 2, BITS == 8)) return -5;
+    // four rows of an output's row are whole 16 (of bfloat16 8) bytes
+    p.bulk_store = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 ? 1 : 0;
     const int row_tiles = GATED ? p.out_chunks * 2 : (p.n + kMsRows - 1) / kMsRows, token_tiles = (p.tokens + BN - 1) / BN, sms = multiprocessor_count();
     const int stages = (p.chunks + MsShape<BITS, BN>::kChunks - 1) / MsShape<BITS, BN>::kChunks;
-    const int wanted = max(1, min(min(sms / (row_tiles * token_tiles), kMsLargestSplit), stages));
+    // Two CTAs fit a multiprocessor: clusters of eight that have one each do not all find room at once (2048 x 8192 and a token: 9.1 us, and 5.0 with room for two),
+    // and a deeper ring gains nothing.  With 128 tokens the sums to be read from eight CTAs cost more than their stages gain (four: 9.1 us, eight: 12.1).
+    const int wanted = max(1, min(min(sms / (row_tiles * token_tiles), BN > 64 ? kMsLargestSplit / 2 : kMsLargestSplit), stages));
     const int per_split = (stages + wanted - 1) / wanted, splits = (stages + per_split - 1) / per_split;   // each has a stage at least
-    int ring = min(per_split, MsSplit<BITS, BN>::kMostStages);
-    // more CTAs than multiprocessors: half the ring, so that two share one
-    if (row_tiles * token_tiles * splits > sms) ring = min(ring, (kMsSplitShared / 2 - 1024 - MsSplit<BITS, BN>::kSlack) / MsShape<BITS, BN>::kStageBytes);
+    const int ring = min(per_split, MsSplit<BITS, BN>::kMostStages);
     auto kernel = gemm_microscaled_split_kernel<BITS, BN, GATED>;
     static OncePerDevice configured;
     if (allow_shared_memory(configured, kernel, kMsSplitShared) != cudaSuccess) return static_cast<int>(cudaGetLastError());

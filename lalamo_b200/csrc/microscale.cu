@@ -7,41 +7,54 @@ namespace lb {
 constexpr int kMicroscaleThreads = 256;
 constexpr int kMicroscaleUnroll = 4;   // pieces of 128 columns that sixteen lanes have in flight
 
-// codes and scales of x [rows, width].  Sixteen lanes take the 128 columns under one word of scales, eight columns each.
+// Division of numbers below 2^31 by one that the host knows: with l = ceil(log2 d) and m = ceil(2^(31 + l) / d), n / d = n m >> (31 + l), exact for those n
+// (m d exceeds 2^(31 + l) by less than d <= 2^l).
+struct Divisor {
+    unsigned divisor, multiplier, shift;
+    __device__ __forceinline__ unsigned quotient(unsigned n) const { return divisor == 1 ? n : __umulhi(n, multiplier) >> shift; }
+};
+inline Divisor divisor_of(unsigned d) {
+    unsigned l = 0;
+    while ((1ull << l) < d) ++l;
+    return {d, d == 1 ? 0u : static_cast<unsigned>(((1ull << (31 + l)) + d - 1) / d), l - 1};
+}
+
+// Pieces of 128 columns under one word of scales, `chunks` of them a row: sixteen lanes take one, eight columns each, and each group of sixteen
+// kMicroscaleUnroll of them.  (There are fewer than 2^31: the rows would not fit the GPU.)
+struct Piece {
+    int row, chunk;
+    bool exists;
+};
+__device__ __forceinline__ Piece piece_of(int u, unsigned total, const Divisor& chunks) {
+    const unsigned piece = blockIdx.x * (kMicroscaleThreads / 16 * kMicroscaleUnroll) + u * (kMicroscaleThreads / 16) + (threadIdx.x >> 4);
+    const unsigned row = chunks.quotient(piece);
+    return {static_cast<int>(row), static_cast<int>(piece - row * chunks.divisor), piece < total};
+}
+
+// codes and scales of x [rows, width]
 template <typename T, int BITS, bool VECTOR>
 __global__ void __launch_bounds__(kMicroscaleThreads)
-microscale_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int rows, int width, int chunks) {
+microscale_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int width, unsigned total, Divisor chunks) {
     wait_for_previous_kernel();
     allow_next_kernel();
-    constexpr int kPieces = kMicroscaleThreads / 16;
-    const long long total = static_cast<long long>(rows) * chunks;
-    const long long first = static_cast<long long>(blockIdx.x) * (kPieces * kMicroscaleUnroll) + (threadIdx.x >> 4);
     const int column = (threadIdx.x & 15) * 8;
+    Piece piece[kMicroscaleUnroll];
     float v[kMicroscaleUnroll][8];
 #pragma unroll
     for (int u = 0; u < kMicroscaleUnroll; ++u) {
-        const long long piece = first + u * kPieces;
-        const long long row = piece / chunks;
-        const int chunk = static_cast<int>(piece - row * chunks);
-        if (piece < total) {
-            load_eight<VECTOR>(x + row * width, chunk * 128 + column, width, v[u]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
-        }
+        piece[u] = piece_of(u, total, chunks);
+        // a piece that does not exist counts as one past its row's width: zeros
+        load_eight<VECTOR>(x + static_cast<size_t>(piece[u].row) * width, piece[u].exists ? piece[u].chunk * 128 + column : width, width, v[u]);
     }
 #pragma unroll
     for (int u = 0; u < kMicroscaleUnroll; ++u) {
-        const long long piece = first + u * kPieces;
-        const long long row = piece / chunks;
-        const int chunk = static_cast<int>(piece - row * chunks);
         uint2 code;
         const uint32_t word = quantise_eight<BITS>(v[u], code);
-        if (piece >= total) continue;
-        const size_t at = static_cast<size_t>(piece) * 128 + column;
+        if (!piece[u].exists) continue;
+        const size_t at = (static_cast<size_t>(piece[u].row) * chunks.divisor + piece[u].chunk) * 128 + column;
         if constexpr (BITS == 8) *reinterpret_cast<uint2*>(codes + at) = code;
         else *reinterpret_cast<uint32_t*>(codes + at / 2) = code.x;
-        if (column == 0) *reinterpret_cast<uint32_t*>(scales + scale_word(static_cast<int>(row), chunk, chunks)) = word;
+        if (column == 0) *reinterpret_cast<uint32_t*>(scales + scale_word(piece[u].row, piece[u].chunk, chunks.divisor)) = word;
     }
 }
 
@@ -49,38 +62,31 @@ microscale_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes, un
 // bfloat16 down to its subnormals).
 template <typename T, int BITS, bool VECTOR>
 __global__ void __launch_bounds__(kMicroscaleThreads)
-microscaled_values_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales, T* __restrict__ out, int rows, int width, int chunks) {
+microscaled_values_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales, T* __restrict__ out, int width, unsigned total, Divisor chunks) {
     wait_for_previous_kernel();
     allow_next_kernel();
-    constexpr int kPieces = kMicroscaleThreads / 16;
-    const long long total = static_cast<long long>(rows) * chunks;
-    const long long first = static_cast<long long>(blockIdx.x) * (kPieces * kMicroscaleUnroll) + (threadIdx.x >> 4);
     const int column = (threadIdx.x & 15) * 8;
+    Piece piece[kMicroscaleUnroll];
     uint2 code[kMicroscaleUnroll];
     int byte[kMicroscaleUnroll];
 #pragma unroll
     for (int u = 0; u < kMicroscaleUnroll; ++u) {
-        const long long piece = first + u * kPieces;
-        if (piece >= total) break;
-        const long long row = piece / chunks;
-        const int chunk = static_cast<int>(piece - row * chunks);
-        const size_t at = static_cast<size_t>(piece) * 128 + column;
+        piece[u] = piece_of(u, total, chunks);
+        if (!piece[u].exists) continue;
+        const size_t at = (static_cast<size_t>(piece[u].row) * chunks.divisor + piece[u].chunk) * 128 + column;
         if constexpr (BITS == 8) code[u] = *reinterpret_cast<const uint2*>(codes + at);
         else code[u].x = *reinterpret_cast<const uint32_t*>(codes + at / 2);
-        byte[u] = scales[scale_word(static_cast<int>(row), chunk, chunks) + column / 32];
+        byte[u] = scales[scale_word(piece[u].row, piece[u].chunk, chunks.divisor) + column / 32];
     }
 #pragma unroll
     for (int u = 0; u < kMicroscaleUnroll; ++u) {
-        const long long piece = first + u * kPieces;
-        if (piece >= total) break;
-        const long long row = piece / chunks;
-        const int chunk = static_cast<int>(piece - row * chunks);
+        if (!piece[u].exists) continue;
         const float scale = scale_value(byte[u]);
         float v[8];
         unpack_eight<BITS>(code[u], v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] *= scale;
-        store_eight<VECTOR>(out + row * width, chunk * 128 + column, width, v);
+        store_eight<VECTOR>(out + static_cast<size_t>(piece[u].row) * width, piece[u].chunk * 128 + column, width, v);
     }
 }
 
@@ -137,23 +143,25 @@ bool rows_are_aligned(const T* rows, int width) {
     return width % 8 == 0 && (reinterpret_cast<uintptr_t>(rows) & 15) == 0;
 }
 
-inline dim3 microscale_grid(int rows, int chunks) {
-    const long long pieces = static_cast<long long>(rows) * chunks, per_block = kMicroscaleThreads / 16 * kMicroscaleUnroll;
-    return dim3(static_cast<unsigned>((pieces + per_block - 1) / per_block));
+inline dim3 microscale_grid(unsigned pieces) {
+    constexpr unsigned per_block = kMicroscaleThreads / 16 * kMicroscaleUnroll;
+    return dim3((pieces + per_block - 1) / per_block);
 }
 
 template <typename T, int BITS>
 cudaError_t launch_microscale(const T* x, unsigned char* codes, unsigned char* scales, int rows, int width, cudaStream_t stream) {
     const int chunks = (width + 127) / 128;
     auto kernel = rows_are_aligned(x, width) ? microscale_kernel<T, BITS, true> : microscale_kernel<T, BITS, false>;
-    return launch_overlapped(kernel, microscale_grid(rows, chunks), dim3(kMicroscaleThreads), 0, stream, x, codes, scales, rows, width, chunks);
+    return launch_overlapped(kernel, microscale_grid(static_cast<unsigned>(rows) * chunks), dim3(kMicroscaleThreads), 0, stream, x, codes, scales, width,
+                             static_cast<unsigned>(rows) * chunks, divisor_of(chunks));
 }
 
 template <typename T, int BITS>
 cudaError_t launch_values(const unsigned char* codes, const unsigned char* scales, T* out, int rows, int width, cudaStream_t stream) {
     const int chunks = (width + 127) / 128;
     auto kernel = rows_are_aligned(out, width) ? microscaled_values_kernel<T, BITS, true> : microscaled_values_kernel<T, BITS, false>;
-    return launch_overlapped(kernel, microscale_grid(rows, chunks), dim3(kMicroscaleThreads), 0, stream, codes, scales, out, rows, width, chunks);
+    return launch_overlapped(kernel, microscale_grid(static_cast<unsigned>(rows) * chunks), dim3(kMicroscaleThreads), 0, stream, codes, scales, out, width,
+                             static_cast<unsigned>(rows) * chunks, divisor_of(chunks));
 }
 
 template <typename TD, int BITS, int GROUPS>
@@ -183,7 +191,7 @@ extern "C" {
 // Return codes: 0, a CUDA error, -1 for an element type, -2 for sizes that the kernels do not take.
 
 int lb_microscale(const void* x, void* codes, void* scales, int rows, int width, int bits, int dtype, cudaStream_t stream) {
-    if (rows < 0 || width < 1 || (bits != 4 && bits != 8)) return -2;
+    if (rows < 0 || width < 1 || (bits != 4 && bits != 8) || static_cast<long long>(rows) * ((width + 127ll) / 128) >= 1ll << 31) return -2;
     if (rows == 0) return 0;
     unsigned char *c = static_cast<unsigned char*>(codes), *s = static_cast<unsigned char*>(scales);
     LB_DISPATCH_DTYPE(dtype, {
@@ -193,7 +201,7 @@ int lb_microscale(const void* x, void* codes, void* scales, int rows, int width,
 }
 
 int lb_microscaled_values(const void* codes, const void* scales, void* out, int rows, int width, int bits, int dtype, cudaStream_t stream) {
-    if (rows < 0 || width < 1 || (bits != 4 && bits != 8)) return -2;
+    if (rows < 0 || width < 1 || (bits != 4 && bits != 8) || static_cast<long long>(rows) * ((width + 127ll) / 128) >= 1ll << 31) return -2;
     if (rows == 0) return 0;
     const unsigned char *c = static_cast<const unsigned char*>(codes), *s = static_cast<const unsigned char*>(scales);
     LB_DISPATCH_DTYPE(dtype, {

@@ -29,7 +29,7 @@ __device__ __forceinline__ int scale_byte(uint32_t largest_bits) {
     return exponent == 255 ? kNoNumber : max(exponent - (BITS == 8 ? 8 : 2), 0);
 }
 
-// One over a scale, exact: the byte of a number is at most 254 - 2.
+// One over a scale, exact: the byte of a number is at most 254 - 2 (and what 255 gives is not looked at).
 __device__ __forceinline__ float scale_inverse(int byte) { return __uint_as_float(static_cast<uint32_t>(254 - byte) << 23); }
 
 // A scale as float32: 2^-127 is a subnormal.
@@ -86,20 +86,26 @@ __device__ __forceinline__ void unpack_eight(uint2 codes, float (&v)[8]) {
     }
 }
 
+// The larger of two magnitudes; a NaN is above all numbers (and stays one with an exponent of all ones).
+__device__ __forceinline__ float larger_size(float a, float b) {
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return c;
+}
+
 // Quantises eight consecutive columns a lane: four lanes hold a block, sixteen the 128 columns under one word of scales.  All lanes of the warp take part.
-// Returns that word (the same in the sixteen lanes); `codes` has eight bytes, or four bytes of halves in codes.x.
+// Returns that word (the same in the sixteen lanes); `codes` has eight bytes, or four bytes of halves in codes.x.  (What the elements of a block
+// are that has no number for a scale says nothing.)
 template <int BITS>
 __device__ __forceinline__ uint32_t quantise_eight(const float (&v)[8], uint2& codes) {
-    uint32_t largest = 0u;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) largest = max(largest, __float_as_uint(v[i]) & 0x7fffffffu);   // as integers: a NaN is above all numbers
-    largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-    largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-    const int byte = scale_byte<BITS>(largest);
-    const float inverse = byte == kNoNumber ? 0.0f : scale_inverse(byte);
+    float largest = larger_size(larger_size(larger_size(v[0], v[1]), larger_size(v[2], v[3])), larger_size(larger_size(v[4], v[5]), larger_size(v[6], v[7])));
+    largest = larger_size(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+    largest = larger_size(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+    const int byte = scale_byte<BITS>(__float_as_uint(largest) & 0x7fffffffu);
+    const float inverse = scale_inverse(byte);
     float scaled[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) scaled[i] = byte == kNoNumber ? 0.0f : v[i] * inverse;
+    for (int i = 0; i < 8; ++i) scaled[i] = v[i] * inverse;
     if constexpr (BITS == 8) {
         codes.x = pack_e4m3(scaled[0], scaled[1], scaled[2], scaled[3]);
         codes.y = pack_e4m3(scaled[4], scaled[5], scaled[6], scaled[7]);
