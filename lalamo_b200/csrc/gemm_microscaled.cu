@@ -51,43 +51,62 @@ __device__ __forceinline__ bool elect_lane() {
 }
 
 // A whole warp waits, and its lanes go on together or not at all.  (Where one lane waited for the others, what the warp issues afterwards took twice as long.)
-__device__ __forceinline__ bool barrier_wait_warp(uint64_t* barrier, uint32_t parity) { return __all_sync(0xffffffffu, barrier_wait_parked(barrier, parity)); }
+// CLUSTER: sees what another CTA did before it arrived.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool barrier_wait_warp(uint64_t* barrier, uint32_t parity) {
+    if constexpr (!CLUSTER) return __all_sync(0xffffffffu, barrier_wait_parked(barrier, parity));
+    bool waited = false;
+    const unsigned long long start = nanoseconds_now();
+    for (;;) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(smem_address(barrier)), "r"(parity), "r"(100000u)
+            : "memory");
+        waited = done != 0u;
+        if (waited || nanoseconds_now() - start > kTcWaitNanoseconds) break;
+    }
+    return __all_sync(0xffffffffu, waited);
+}
 
 // A tile of scales, 32 rows of 16 bytes one behind the other (groups of 8 rows 128 bytes apart, no swizzle), for tcgen05.cp.
 __device__ __forceinline__ uint64_t scale_descriptor(const void* tile) {
     const uint64_t address = smem_address(tile);
     return ((address & 0x3FFFFull) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) | (1ull << 46);
 }
-// To four columns of tensor memory, the same in each quarter of the lanes.
+// To four columns of tensor memory, the same in each quarter of the lanes.  PAIR: each CTA of the pair from its own shared memory, at the same place.
+template <bool PAIR>
 __device__ __forceinline__ void copy_scales(uint32_t tmem, const void* tile) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(scale_descriptor(tile)) : "memory");
+    if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(scale_descriptor(tile)) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(scale_descriptor(tile)) : "memory");
 }
 
-// D float32 [128, N] (+)= A [128, 32] e2m1 (spread) B [N, 32] e4m3, or A [128, 64] e2m1 B [N, 64] e2m1, each block of 32 times its two scales.
-template <int BITS>
+// D float32 [128, N] (+)= A [128, 32] e2m1 (spread) B [N, 32] e4m3, or A [128, 64] e2m1 B [N, 64] e2m1, each block of 32 times its two scales.  PAIR: [256, N] over two
+// CTAs, each with 128 rows of A and of D, half of the rows of B, its rows' scales and all of the tokens'.
+#define LB_MMA_MICROSCALED(group, kind, scales)                                                                                                    \
+    asm volatile(                                                                                                                                  \
+        "{\n\t.reg .pred p;\n\t"                                                                                                                  \
+        "setp.ne.b32 p, %4, 0;\n\t"                                                                                                               \
+        "tcgen05.mma.cta_group::" group ".kind::" kind ".block_scale.scale_vec::" scales " [%0], %1, %2, %3, [%5], [%6], p;\n\t}"                 \
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(scales_a), "r"(scales_b)                                \
+        : "memory")
+template <int BITS, bool PAIR>
 __device__ __forceinline__ void mma_microscaled(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t scales_a, uint32_t scales_b, bool accumulate) {
-    if constexpr (BITS == 8) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
-            ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(scales_a), "r"(scales_b)
-            : "memory");
-    } else {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
-            ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(scales_a), "r"(scales_b)
-            : "memory");
-    }
+    if constexpr (BITS == 8 && PAIR) LB_MMA_MICROSCALED("2", "mxf8f6f4", "1X");
+    else if constexpr (BITS == 8) LB_MMA_MICROSCALED("1", "mxf8f6f4", "1X");
+    else if constexpr (PAIR) LB_MMA_MICROSCALED("2", "mxf4", "2X");
+    else LB_MMA_MICROSCALED("1", "mxf4", "2X");
 }
+#undef LB_MMA_MICROSCALED
 
-// The instruction's description: A (W) e2m1, B (X) e4m3 or e2m1, scales e8m0, N columns, 128 lanes; the bytes of the scales' words follow per product.
+// The instruction's description: A (W) e2m1, B (X) e4m3 or e2m1, scales e8m0, N columns, 128 lanes (a pair's 256); the bytes of the scales' words follow per product.
 template <int BITS>
-__device__ __forceinline__ uint32_t microscaled_descriptor(int columns) {
+__device__ __forceinline__ uint32_t microscaled_descriptor(int columns, int lanes = kMsRows) {
     const uint32_t types = BITS == 8 ? (5u << 7) | (0u << 10) : (1u << 7) | (1u << 10);
-    return types | (static_cast<uint32_t>(columns >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(kMsRows >> 4) << 24);
+    return types | (static_cast<uint32_t>(columns >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(lanes >> 4) << 24);
 }
 // Product `k` of the four of a stage takes the scales from this chunk of the stage, and from this byte on of its words.
 template <int BITS>
@@ -112,13 +131,13 @@ __device__ __forceinline__ float ms_up_side(float u, int activation, float limit
     return activation == kSigmoidLimit ? fminf(fmaxf(u, -limit), limit) + 1.0f : u;
 }
 
-// BN: tokens of a tile.  A tile of more than 128 begins at a multiple of 64, so that two tiles of scales cover it.
-template <int BITS, int BN>
+// BN: tokens of a tile, of which a CTA loads OWN.  A tile of more than 128 begins at a multiple of 64, so that two tiles of scales cover it.
+template <int BITS, int BN, int OWN = BN>
 struct MsShape {
     static constexpr int kChunks = BITS == 8 ? 1 : 2;             // of 128 columns, a stage
     static constexpr int kScaleTiles = BN > 128 ? 2 : 1;          // of 128 tokens, that a tile's tokens lie in
     static constexpr int kWBytes = kMsRows * 128;
-    static constexpr int kXBytes = BN * 128;
+    static constexpr int kXBytes = OWN * 128;
     static constexpr int kWScaleBytes = kChunks * kScaleTileBytes;
     static constexpr int kXScaleBytes = kScaleTiles * kChunks * kScaleTileBytes;
     static constexpr int kStageBytes = (kWBytes + kXBytes + kWScaleBytes + kXScaleBytes + 1023) / 1024 * 1024;   // tiles start on 1024 bytes
@@ -126,29 +145,33 @@ struct MsShape {
     static constexpr uint32_t kWCounted = BITS == 8 ? kWBytes / 2 : kWBytes;
 };
 
-// One lane's work on a stage that has landed, of `chunks` 128s: its scales to tensor memory, its four products, and the stage's return to the producer.
-template <int BITS, int BN>
-__device__ __forceinline__ void issue_stage(uint32_t tmem_d, const unsigned char* stage, uint32_t columns, uint32_t token_column, uint32_t idesc, int chunks, bool accumulate,
-                                            uint64_t* empty) {
-    using Shape = MsShape<BITS, BN>;
+// One lane's work: a landed stage's scales to a set of columns of tensor memory,
+template <typename Shape, bool PAIR>
+__device__ __forceinline__ void copy_stage_scales(const unsigned char* stage, uint32_t columns, int chunks) {
     const unsigned char* scales = stage + Shape::kWBytes + Shape::kXBytes;
 #pragma unroll
     for (int c = 0; c < Shape::kChunks; ++c) {
         if (c >= chunks) break;
-        copy_scales(columns + 4 * c, scales + c * kScaleTileBytes);
+        copy_scales<PAIR>(columns + 4 * c, scales + c * kScaleTileBytes);
 #pragma unroll
         for (int t = 0; t < Shape::kScaleTiles; ++t)
-            copy_scales(columns + 4 * (Shape::kChunks + c * Shape::kScaleTiles + t), scales + Shape::kWScaleBytes + (t * Shape::kChunks + c) * kScaleTileBytes);
+            copy_scales<PAIR>(columns + 4 * (Shape::kChunks + c * Shape::kScaleTiles + t), scales + Shape::kWScaleBytes + (t * Shape::kChunks + c) * kScaleTileBytes);
     }
+}
+// and its four products under them, and the stage's return to the producer(s).
+template <int BITS, typename Shape, bool PAIR>
+__device__ __forceinline__ void issue_stage(uint32_t tmem_d, const unsigned char* stage, uint32_t columns, uint32_t token_column, uint32_t idesc, int chunks, bool accumulate,
+                                            uint64_t* empty) {
     const uint64_t desc_w = tile_descriptor(stage), desc_x = tile_descriptor(stage + Shape::kWBytes);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int c = product_chunk<BITS>(k);
         if (c >= chunks) break;
-        mma_microscaled<BITS>(tmem_d, desc_w + 2 * k, desc_x + 2 * k, idesc | product_scales<BITS>(k), columns + 4 * c,
-                              columns + 4 * (Shape::kChunks + c * Shape::kScaleTiles) + token_column, accumulate || k > 0);
+        mma_microscaled<BITS, PAIR>(tmem_d, desc_w + 2 * k, desc_x + 2 * k, idesc | product_scales<BITS>(k), columns + 4 * c,
+                                    columns + 4 * (Shape::kChunks + c * Shape::kScaleTiles) + token_column, accumulate || k > 0);
     }
-    mma_commit(empty);
+    if constexpr (PAIR) mma_commit_pair(empty);
+    else mma_commit(empty);
 }
 
 constexpr int kMsThreads = 20 * 32;             // producer, issuer, scales of a gated product, one idle; sixteen warps of the epilogue
@@ -159,24 +182,33 @@ constexpr int kMsRegionBytes = 11 * 1024;       // per four warps: gated, 16 tok
 static_assert(kMsRegionBytes >= kMsTurnedBytes + 2 * kMsGroup * 64 && kMsRegionBytes >= kMsGroup * kMsRows * 4, "room for either");
 constexpr int kMsSharedLimit = 227 * 1024;
 
-template <int BITS, int BN>
+template <int BITS, int BN, bool PAIR>
 struct MsWalk {
-    static constexpr int kStages = (kMsSharedLimit - 4 * kMsRegionBytes - 1024 - 256) / MsShape<BITS, BN>::kStageBytes;
-    static constexpr int kBytes = kStages * MsShape<BITS, BN>::kStageBytes + 4 * kMsRegionBytes + 1024 + 256;
-    static constexpr int kScaleColumns = 4 * MsShape<BITS, BN>::kChunks * (1 + MsShape<BITS, BN>::kScaleTiles);
+    using Shape = MsShape<BITS, BN, PAIR ? BN / 2 : BN>;
+    static constexpr int kStages = (kMsSharedLimit - 4 * kMsRegionBytes - 1024 - 256) / Shape::kStageBytes;
+    static constexpr int kBytes = kStages * Shape::kStageBytes + 4 * kMsRegionBytes + 1024 + 256;
+    static constexpr int kScaleSet = 4 * Shape::kChunks * (1 + Shape::kScaleTiles);
+    static constexpr int kScaleColumns = (PAIR ? 2 : 1) * kScaleSet;
     static constexpr int kColumns = 2 * BN + kScaleColumns <= 256 ? 256 : 512;
     static_assert(kStages >= 3 && kStages <= 12 && 2 * BN + kScaleColumns <= 512, "a ring, its barriers, two accumulators and the scales");
 };
 
 // One CTA per multiprocessor walks the tiles of 128 lanes x BN tokens, rows fastest, with two accumulators: the epilogue of a tile runs while the
-// products of the next are issued.
-template <int BITS, int BN, bool GATED>
+// products of the next are issued.  PAIR: the walkers are pairs of CTAs that share a tile of 256 lanes; each loads its rows of W, half of the tokens and all
+// of their scales, all bytes count on the even CTA's barriers, and that one issues products over both CTAs' shared and tensor memory.  (Not for gated products,
+// whose scales would have to be announced across the pair, nor rows of 4 bits: 4096 x 8192 x 2048 40.3 us and 38.0 without.)
+template <int BITS, int BN, bool GATED, bool PAIR>
 __global__ void __launch_bounds__(kMsThreads)
 gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_gate, const __grid_constant__ CUtensorMap map_x,
-                        const __grid_constant__ CUtensorMap map_out, const MsParams p) {
-    using Shape = MsShape<BITS, BN>;
-    using Walk = MsWalk<BITS, BN>;
+                        const __grid_constant__ CUtensorMap map_w_scales, const __grid_constant__ CUtensorMap map_x_scales, const __grid_constant__ CUtensorMap map_out,
+                        const MsParams p) {
+    static_assert(!PAIR || (BITS == 8 && !GATED), "what pairs take");
+    using Walk = MsWalk<BITS, BN, PAIR>;
+    using Shape = typename Walk::Shape;
     constexpr int STAGES = Walk::kStages;
+    constexpr int kPairs = PAIR ? 2 : 1;   // CTAs of a walker
+    const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
+    const int walker = static_cast<int>(blockIdx.x) / kPairs, walkers = static_cast<int>(gridDim.x) / kPairs;
     extern __shared__ unsigned char raw_shared[];
     unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_shared) + 1023) & ~static_cast<uintptr_t>(1023));
     unsigned char* regions = ring + STAGES * Shape::kStageBytes;
@@ -189,10 +221,12 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     __shared__ int failed;
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    constexpr int kRowsPerTile = GATED ? kMsRows / 2 : kMsRows;
+    constexpr int kRowsPerCta = GATED ? kMsRows / 2 : kMsRows;
     const int num_stages = (p.chunks + Shape::kChunks - 1) / Shape::kChunks;
     const int num_tiles = p.row_tiles * p.token_tiles;
     auto chunks_of = [&](int stage) { return min(Shape::kChunks, p.chunks - stage * Shape::kChunks); };
+    auto row_of = [&](int tile) { return ((tile % p.row_tiles) * kPairs + rank) * kRowsPerCta; };   // this CTA's first
+    auto token_of = [&](int tile) { return tile / p.row_tiles * BN; };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -201,17 +235,23 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         }
         for (int a = 0; a < 2; ++a) {
             barrier_init(&tmem_full[a], 1);
-            barrier_init(&tmem_empty[a], 16);
+            barrier_init(&tmem_empty[a], 16 * kPairs);
         }
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(tmem_slot)), "r"(Walk::kColumns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(tmem_slot)), "r"(Walk::kColumns) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(tmem_slot)), "r"(Walk::kColumns) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();   // the partner's barriers exist before anything arrives on them
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t tmem_scales = tmem_base + 2 * BN;
@@ -222,13 +262,10 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     if (warp == 0) {
         int s = 0, round = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-            const int row0 = (tile % p.row_tiles) * kRowsPerTile, token0 = (tile / p.row_tiles) * BN;
-            const int scale_tiles = min(Shape::kScaleTiles, (p.tokens + 127) / 128 - token0 / 128);
-            const unsigned char* w_scales = p.w_scales + static_cast<size_t>(row0 / 128) * p.chunks * kScaleTileBytes;
-            const unsigned char* x_scales = p.x_scales + static_cast<size_t>(token0 / 128) * p.chunks * kScaleTileBytes;
+        for (int tile = walker; tile < num_tiles && ok; tile += walkers) {
+            const int row0 = row_of(tile), token0 = token_of(tile);
             for (int stage = 0; stage < num_stages; ++stage) {
-                ok = round == 0 || barrier_wait_warp(&empty[s], (round - 1) & 1);
+                ok = round == 0 || barrier_wait_warp<PAIR>(&empty[s], (round - 1) & 1);
                 if (!ok) {
                     atomicExch(&failed, 1);
                     break;
@@ -236,47 +273,83 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                 if (elect_lane()) {
                     unsigned char* at = ring + s * Shape::kStageBytes;
                     const int column = stage * 128;   // of the map: elements of W where they are spread and of X in 8 bits, bytes of rows in 4
-                    const int chunk = stage * Shape::kChunks;
-                    const uint32_t scale_bytes = static_cast<uint32_t>(chunks_of(stage) * kScaleTileBytes);
-                    barrier_expect(&full[s], Shape::kWCounted + Shape::kXBytes + (GATED ? 0u : scale_bytes) + scale_tiles * scale_bytes);
-                    tma_load_2d(at, &map_w, column, row0, &full[s]);
-                    if constexpr (GATED) tma_load_2d(at + Shape::kWBytes / 2, &map_gate, column, row0, &full[s]);
-                    tma_load_2d(at + Shape::kWBytes, &map_x, column, token0, &full[s]);
+                    const int word = stage * Shape::kChunks * (kScaleTileBytes / 4);
+                    if (rank == 0) barrier_expect(&full[s], kPairs * (Shape::kWCounted + Shape::kXBytes + (GATED ? 0 : Shape::kWScaleBytes) + Shape::kXScaleBytes));
+                    auto load = [&](void* to, const CUtensorMap* map, int x, int y) {
+                        if constexpr (PAIR) tma_load_2d_pair(to, map, x, y, cluster_address(&full[s], 0));
+                        else tma_load_2d(to, map, x, y, &full[s]);
+                    };
+                    load(at, &map_w, column, row0);
+                    if constexpr (GATED) load(at + Shape::kWBytes / 2, &map_gate, column, row0);
+                    load(at + Shape::kWBytes, &map_x, column, token0 + rank * (BN / 2));
                     at += Shape::kWBytes + Shape::kXBytes;
-                    if constexpr (!GATED) bulk_load(at, w_scales + static_cast<size_t>(chunk) * kScaleTileBytes, scale_bytes, &full[s]);
-                    at += Shape::kWScaleBytes;
-                    for (int t = 0; t < scale_tiles; ++t)
-                        bulk_load(at + t * Shape::kWScaleBytes, x_scales + (static_cast<size_t>(t) * p.chunks + chunk) * kScaleTileBytes, scale_bytes, &full[s]);
+                    if constexpr (!GATED) load(at, &map_w_scales, word, row0 / 128);
+                    load(at + Shape::kWScaleBytes, &map_x_scales, word, token0 / 128);
                 }
                 if (++s == STAGES) s = 0, ++round;
             }
         }
     } else if (warp == 1) {
-        const uint32_t idesc = microscaled_descriptor<BITS>(BN);
-        int s = 0, round = 0, local = 0;
-        bool ok = true;
-        for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++local) {
+        const uint32_t idesc = microscaled_descriptor<BITS>(BN, kPairs * kMsRows);
+        int s = 0, round = 0, local = 0, left = (num_tiles - walker + walkers - 1) / walkers * num_stages;
+        uint32_t set = 0u;
+        bool ok = rank == 0, copied = false;
+        for (int tile = walker; tile < num_tiles && ok; tile += walkers, ++local) {
             const int accumulator = local & 1, use = local >> 1;
-            ok = use == 0 || barrier_wait_warp(&tmem_empty[accumulator], (use - 1) & 1);
+            ok = use == 0 || barrier_wait_warp<PAIR>(&tmem_empty[accumulator], (use - 1) & 1);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(accumulator * BN);
-            const uint32_t token_column = static_cast<uint32_t>((((tile / p.row_tiles) * BN) & 127) >> 5);   // of the scales: 32 tokens a column
+            const uint32_t token_column = static_cast<uint32_t>((token_of(tile) & 127) >> 5);   // of the scales: 32 tokens a column
             for (int stage = 0; stage < num_stages && ok; ++stage) {
-                ok = barrier_wait_warp(&full[s], round & 1);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (elect_lane()) issue_stage<BITS, BN>(tmem_d, ring + s * Shape::kStageBytes, tmem_scales, token_column, idesc, chunks_of(stage), stage > 0, &empty[s]);
-                if (++s == STAGES) s = 0, ++round;
+                const unsigned char* at = ring + s * Shape::kStageBytes;
+                if constexpr (!PAIR) {
+                    ok = barrier_wait_warp(&full[s], round & 1);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    // In one branch or in two: with rows of 8 bits two are sooner done (2048 tokens, 2048 x 8192: 35.9 us and 38.0), with 4 bits one (20.6 and 22.6).
+                    if constexpr (BITS == 8) {
+                        if (elect_lane()) copy_stage_scales<Shape, false>(at, tmem_scales, chunks_of(stage));
+                        if (elect_lane()) issue_stage<BITS, Shape, false>(tmem_d, at, tmem_scales, token_column, idesc, chunks_of(stage), stage > 0, &empty[s]);
+                    } else if (elect_lane()) {
+                        copy_stage_scales<Shape, false>(at, tmem_scales, chunks_of(stage));
+                        issue_stage<BITS, Shape, false>(tmem_d, at, tmem_scales, token_column, idesc, chunks_of(stage), stage > 0, &empty[s]);
+                    }
+                    if (++s == STAGES) s = 0, ++round;
+                } else {
+                    // A pair's scales of the stage after go out before this stage's products if that stage is there (4096 tokens x 2048 x 8192: 60.8 us, and 65.4 with
+                    // copies just before their products; a CTA by itself does not gain by it, 69.1 and 68.4).
+                    const uint32_t columns = tmem_scales + set * Walk::kScaleSet;
+                    if (!copied) {
+                        ok = barrier_wait_warp<true>(&full[s], round & 1);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (elect_lane()) copy_stage_scales<Shape, true>(at, columns, chunks_of(stage));
+                    }
+                    const int next = s + 1 == STAGES ? 0 : s + 1, next_round = s + 1 == STAGES ? round + 1 : round;
+                    copied = --left > 0 && __all_sync(0xffffffffu, barrier_test(&full[next], next_round & 1));
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (elect_lane()) {
+                        if (copied)
+                            copy_stage_scales<Shape, true>(ring + next * Shape::kStageBytes, tmem_scales + (set ^ 1u) * Walk::kScaleSet, chunks_of(stage + 1 == num_stages ? 0 : stage + 1));
+                        issue_stage<BITS, Shape, true>(tmem_d, at, columns, token_column, idesc, chunks_of(stage), stage > 0, &empty[s]);
+                    }
+                    s = next, round = next_round, set ^= 1u;
+                }
             }
-            if (!ok) atomicExch(&failed, 1);
-            else if (elect_lane()) mma_commit(&tmem_full[accumulator]);
+            if (!ok) {
+                atomicExch(&failed, 1);
+            } else if (elect_lane()) {
+                if constexpr (PAIR) mma_commit_pair(&tmem_full[accumulator]);
+                else mma_commit(&tmem_full[accumulator]);
+            }
         }
     } else if (GATED && warp == 2) {
         // Lane l puts together the 16 bytes of the rows l, l + 32 of `up` and of `gate` in the accumulator's order.  Four stages are read at once: a
         // read from L2 takes about as long as the products of two.
-        int issued = 0;
+        int s = 0, round = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-            const int row0 = (tile % p.row_tiles) * kRowsPerTile;
+        for (int tile = walker; tile < num_tiles && ok; tile += walkers) {
+            const int row0 = row_of(tile);
             const size_t offset = static_cast<size_t>(row0 / 128) * p.chunks * kScaleTileBytes + lane * 16 + ((row0 & 64) >> 3);
             for (int first = 0; first < num_stages && ok; first += 4) {
                 uint2 up[4][Shape::kChunks], gate[4][Shape::kChunks];
@@ -295,7 +368,6 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if (first + i >= num_stages) break;
-                    const int s = issued % STAGES, round = issued / STAGES;
                     ok = round == 0 || barrier_wait_warp(&empty[s], (round - 1) & 1);
                     if (!ok) {
                         atomicExch(&failed, 1);
@@ -308,7 +380,7 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) barrier_arrive(&full[s]);
-                    ++issued;
+                    if (++s == STAGES) s = 0, ++round;
                 }
             }
         }
@@ -318,10 +390,10 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         const bool issuer = quarter == 0 && lane == 0;
         unsigned char* region = regions + set * kMsRegionBytes;
         int local = 0, groups = 0;
-        for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++local) {
+        for (int tile = walker; tile < num_tiles; tile += walkers, ++local) {
             const int accumulator = local & 1, use = local >> 1;
-            const int row0 = (tile % p.row_tiles) * kRowsPerTile, token0 = (tile / p.row_tiles) * BN;
-            uint32_t arrived = barrier_wait_warp(&tmem_full[accumulator], use & 1) ? 1u : 0u;
+            const int row0 = row_of(tile), token0 = token_of(tile);
+            uint32_t arrived = barrier_wait_warp<PAIR>(&tmem_full[accumulator], use & 1) ? 1u : 0u;
             {
                 // Warps that meet at named barriers below go on together or not at all.
                 uint32_t all;
@@ -426,7 +498,10 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) barrier_arrive(&tmem_empty[accumulator]);
+            if (lane == 0) {
+                if constexpr (PAIR) barrier_arrive_cluster(cluster_address(&tmem_empty[accumulator], 0));
+                else barrier_arrive(&tmem_empty[accumulator]);
+            }
         }
         if (issuer) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
@@ -438,7 +513,12 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         for (int spin = 0; spin < 2000; ++spin) __nanosleep(1000);
         __syncthreads();
     }
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Walk::kColumns) : "memory");
+    // PAIR: neither CTA leaves, or gives its tensor memory back, while the other may still touch them.
+    if constexpr (PAIR) cluster_sync();
+    if (warp == 1) {
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Walk::kColumns) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Walk::kColumns) : "memory");
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -544,8 +624,11 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
             ok = barrier_wait_warp(&full[s], round & 1);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (elect_lane())
-                issue_stage<BITS, BN>(tmem_base, ring + s * Shape::kStageBytes, tmem_base + BN, static_cast<uint32_t>((token0 & 127) >> 5), idesc, chunks_of(first_stage + i), i > 0, &empty[s]);
+            if (elect_lane()) {
+                const unsigned char* at = ring + s * Shape::kStageBytes;
+                copy_stage_scales<Shape, false>(at, tmem_base + BN, chunks_of(first_stage + i));
+                issue_stage<BITS, Shape, false>(tmem_base, at, tmem_base + BN, static_cast<uint32_t>((token0 & 127) >> 5), idesc, chunks_of(first_stage + i), i > 0, &empty[s]);
+            }
             if (++s == ring_stages) s = 0, ++round;
         }
         if (!ok) atomicExch(&failed, 1);
@@ -723,31 +806,65 @@ static bool make_ms_out_map(CUtensorMap* map, void* base, int tokens, int width,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BITS, int BN, bool GATED>
+// Scales as boxes of [tiles, chunks] of them, in words.
+static bool make_scales_map(CUtensorMap* map, const void* scales, int row_tiles, int chunks, int box_tiles, int box_chunks) {
+    EncodeTiled encode = encode_tiled();
+    if (encode == nullptr) return false;
+    constexpr cuuint32_t words = kScaleTileBytes / 4;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(chunks) * words, static_cast<cuuint64_t>(row_tiles)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(chunks) * kScaleTileBytes};
+    const cuuint32_t box[2] = {box_chunks * words, static_cast<cuuint32_t>(box_tiles)};
+    const cuuint32_t element_strides[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(scales), dims, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BITS, int BN, bool GATED, bool PAIR>
 int launch_microscaled(const void* x, const void* w, const void* gate, MsParams p, cudaStream_t stream) {
-    CUtensorMap map_w, map_gate, map_x, map_out;
+    using Walk = MsWalk<BITS, BN, PAIR>;
+    using Shape = typename Walk::Shape;
+    CUtensorMap map_w, map_gate, map_x, map_w_scales, map_x_scales, map_out;
     const int w_bytes = p.chunks * 64, x_bytes = p.chunks * 16 * BITS;
-    if (!make_codes_map(&map_w, w, p.n, w_bytes, GATED ? kMsRows / 2 : kMsRows, BITS == 8) || !make_codes_map(&map_x, x, p.tokens, x_bytes, BN, false)) return -5;
+    if (!make_codes_map(&map_w, w, p.n, w_bytes, GATED ? kMsRows / 2 : kMsRows, BITS == 8) || !make_codes_map(&map_x, x, p.tokens, x_bytes, PAIR ? BN / 2 : BN, false) ||
+        !make_scales_map(&map_w_scales, p.w_scales, (p.n + 127) / 128, p.chunks, 1, Shape::kChunks) ||
+        !make_scales_map(&map_x_scales, p.x_scales, (p.tokens + 127) / 128, p.chunks, Shape::kScaleTiles, Shape::kChunks))
+        return -5;
     map_gate = map_w, map_out = map_x;
+    int row_tiles;
     if constexpr (GATED) {
         if (!make_codes_map(&map_gate, gate, p.n, w_bytes, kMsRows / 2, BITS == 8) ||
             !make_ms_out_map(&map_out, p.out, p.tokens, p.out_chunks * 128, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, kMsRows / 2, kMsGroup))
             return -5;
-        p.row_tiles = p.out_chunks * 2;
+        row_tiles = p.out_chunks * 2;
     } else {
         const int size = p.out_is_float ? 4 : 2;
         p.bulk_store = (static_cast<size_t>(p.n) * size) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 ? 1 : 0;
         if (p.bulk_store && !make_ms_out_map(&map_out, p.out, p.tokens, p.n, p.out_is_float ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, size,
                                              kMsRows, kMsGroup))
             return -5;
-        p.row_tiles = (p.n + kMsRows - 1) / kMsRows;
+        row_tiles = (p.n + kMsRows - 1) / kMsRows;
     }
+    p.row_tiles = PAIR ? (row_tiles + 1) / 2 : row_tiles;
     p.token_tiles = (p.tokens + BN - 1) / BN;
-    auto kernel = gemm_microscaled_kernel<BITS, BN, GATED>;
+    auto kernel = gemm_microscaled_kernel<BITS, BN, GATED, PAIR>;
     static OncePerDevice configured;
-    if (allow_shared_memory(configured, kernel, MsWalk<BITS, BN>::kBytes) != cudaSuccess) return static_cast<int>(cudaGetLastError());
-    const int tiles = p.row_tiles * p.token_tiles, sms = multiprocessor_count();
-    return static_cast<int>(launch_overlapped(kernel, dim3(tiles < sms ? tiles : sms), dim3(kMsThreads), MsWalk<BITS, BN>::kBytes, stream, map_w, map_gate, map_x, map_out, p));
+    if (allow_shared_memory(configured, kernel, Walk::kBytes) != cudaSuccess) return static_cast<int>(cudaGetLastError());
+    const int tiles = p.row_tiles * p.token_tiles, walkers = multiprocessor_count() / (PAIR ? 2 : 1);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((tiles < walkers ? tiles : walkers) * (PAIR ? 2 : 1));
+    config.blockDim = dim3(kMsThreads);
+    config.dynamicSmemBytes = Walk::kBytes;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = overlap_launches() ? 1 : 0;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = 2;
+    attributes[1].val.clusterDim.y = 1;
+    attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = PAIR ? 2 : 1;
+    return static_cast<int>(cudaLaunchKernelEx(&config, kernel, map_w, map_gate, map_x, map_w_scales, map_x_scales, map_out, p));
 }
 
 template <int BITS, int BN, bool GATED>
@@ -786,16 +903,27 @@ int launch_microscaled_split(const void* x, const void* w, const void* gate, MsP
     return static_cast<int>(cudaLaunchKernelEx(&config, kernel, map_w, map_gate, map_x, p, splits, per_split, ring));
 }
 
-// Which kernel: tiles of 128 rows x 192 tokens that fill the multiprocessors are walked; fewer are cut along K.
+// Which kernel.  Few tiles are cut along K: up to 128 tokens, and up to half of the multiprocessors in tiles of 128 x 128.  Else the tiles are walked, and what decides is
+// how many rounds of tiles a walker has and what a stage of K costs in each (measured under sustained load at 4,096 tokens, 2048 x 8192: 0.29 us with 128 tokens a
+// tile, 0.36 with 192, 0.32 of a pair with 192), a pair some 2.5 us at the start.  With 2,048 tokens and 2048 x 2048 tiles of 128 tokens take 11.7 us,
+// of 192 13.1 and pairs 13.8; with 777 and 6912 x 1536 12.8, 11.7 and 11.1.
 template <int BITS, bool GATED>
 int launch_microscaled_tiles(const void* x, const void* w, const void* gate, const MsParams& p, cudaStream_t stream) {
-    const int row_tiles = GATED ? p.out_chunks * 2 : (p.n + kMsRows - 1) / kMsRows, sms = multiprocessor_count();
+    const long long row_tiles = GATED ? p.out_chunks * 2 : (p.n + kMsRows - 1) / kMsRows, narrow = row_tiles * ((p.tokens + 127) / 128);
+    const int sms = multiprocessor_count();
     if (p.tokens <= 16) return launch_microscaled_split<BITS, 16, GATED>(x, w, gate, p, stream);
     if (p.tokens <= 32) return launch_microscaled_split<BITS, 32, GATED>(x, w, gate, p, stream);
     if (p.tokens <= 64) return launch_microscaled_split<BITS, 64, GATED>(x, w, gate, p, stream);
-    if (p.tokens <= 128 || row_tiles * ((p.tokens + 127) / 128) <= sms / 2) return launch_microscaled_split<BITS, 128, GATED>(x, w, gate, p, stream);
-    if (row_tiles * ((p.tokens + 127) / 128) <= sms) return launch_microscaled<BITS, 128, GATED>(x, w, gate, p, stream);
-    return launch_microscaled<BITS, 192, GATED>(x, w, gate, p, stream);
+    if (p.tokens <= 128 || narrow <= sms / 2) return launch_microscaled_split<BITS, 128, GATED>(x, w, gate, p, stream);
+    const int wide_tokens = (p.tokens + 191) / 192;
+    const long long stages = (p.chunks + MsShape<BITS, 128>::kChunks - 1) / MsShape<BITS, 128>::kChunks;
+    const long long narrow_cost = (narrow + sms - 1) / sms * stages * 29, wide_cost = (row_tiles * wide_tokens + sms - 1) / sms * stages * 36;
+    if constexpr (BITS == 8 && !GATED) {
+        const long long pairs = sms / 2, pair_cost = ((row_tiles + 1) / 2 * wide_tokens + pairs - 1) / pairs * stages * 32 + 250;
+        if (pair_cost < narrow_cost && pair_cost < wide_cost) return launch_microscaled<BITS, 192, GATED, true>(x, w, gate, p, stream);
+    }
+    if (narrow_cost < wide_cost) return launch_microscaled<BITS, 128, GATED, false>(x, w, gate, p, stream);
+    return launch_microscaled<BITS, 192, GATED, false>(x, w, gate, p, stream);
 }
 
 }  // namespace lb
