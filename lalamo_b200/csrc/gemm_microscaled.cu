@@ -880,7 +880,10 @@ int launch_microscaled_split(const void* x, const void* w, const void* gate, MsP
     const int stages = (p.chunks + MsShape<BITS, BN>::kChunks - 1) / MsShape<BITS, BN>::kChunks;
     // Two CTAs fit a multiprocessor: clusters of eight that have one each do not all find room at once (2048 x 8192 and a token: 9.1 us, and 5.0 with room for two),
     // and a deeper ring gains nothing.  With 128 tokens the sums to be read from eight CTAs cost more than their stages gain (four: 9.1 us, eight: 12.1).
-    const int wanted = max(1, min(min(sms / (row_tiles * token_tiles), BN > 64 ? kMsLargestSplit / 2 : kMsLargestSplit), stages));
+    int wanted = max(1, min(min(sms / (row_tiles * token_tiles), BN > 64 ? kMsLargestSplit / 2 : kMsLargestSplit), stages));
+    // Gated tiles that nearly fill the multiprocessors are cut in two all the same, two CTAs to each (8192 x 2048, 64 tokens: 11.3 and 9.4 us; other products lose
+    // by it: 6.4 and 7.3).
+    if (GATED && wanted == 1 && stages > 1 && row_tiles * token_tiles <= sms && (BITS == 8 || BN > 16)) wanted = 2;
     const int per_split = (stages + wanted - 1) / wanted, splits = (stages + per_split - 1) / per_split;   // each has a stage at least
     const int ring = min(per_split, MsSplit<BITS, BN>::kMostStages);
     auto kernel = gemm_microscaled_split_kernel<BITS, BN, GATED>;

@@ -2548,15 +2548,15 @@ class Microscaled:
     :func:`microscale` and :func:`rmsnorm_microscaled` make them, :func:`linear_microscaled` and :func:`gated_linear_microscaled` read them;
     :meth:`values` gives the numbers back.  Tensors that do not fit this are refused here."""
 
-    __slots__ = ("_codes", "_scales", "_store", "bits", "chunks", "device_index", "rows", "width")
+    __slots__ = ("_codes", "_scales", "_scales_at", "_store", "bits", "chunks", "device_index", "rows", "width")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, width: int, bits: int) -> None:
         if bits != 8 and bits != 4:
             raise KernelError(f"Microscaled: elements have 4 or 8 bits, not {bits}")
-        chunks = -(-width // 128)
-        if width < 1 or codes.dim() != 2 or codes.shape[1] != chunks * 16 * bits:
-            raise KernelError(f"Microscaled: codes of shape {tuple(codes.shape)} are not rows of {width} elements of {bits} bits, made up to whole 128s")
-        rows = codes.shape[0]
+        chunks, shape = -(-width // 128), codes.shape
+        if width < 1 or len(shape) != 2 or shape[1] != chunks * 16 * bits:
+            raise KernelError(f"Microscaled: codes of shape {tuple(shape)} are not rows of {width} elements of {bits} bits, made up to whole 128s")
+        rows = shape[0]
         if scales.shape != (-(-rows // 128), chunks, 512):
             raise KernelError(f"Microscaled: scales of shape {tuple(scales.shape)} do not belong to {rows} rows of {width} elements")
         if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or not codes.is_contiguous() or not scales.is_contiguous():
@@ -2566,7 +2566,7 @@ class Microscaled:
             raise KernelError("Microscaled: codes and scales must live on one CUDA device (there is no CPU path)")
         if codes.data_ptr() % 32 or scales.data_ptr() % 16:
             raise KernelError("Microscaled: codes start on 32 bytes and scales on 16")
-        self._codes, self._scales, self._store = codes, scales, None
+        self._codes, self._scales, self._store, self._scales_at = codes, scales, None, 0
         self.rows, self.width, self.bits, self.chunks, self.device_index = rows, width, bits, chunks, device
 
     @classmethod
@@ -2575,15 +2575,15 @@ class Microscaled:
         made when somebody asks for them; two allocations and the checks above took 5 us of a call of 10."""
         self = cls.__new__(cls)
         chunks = -(-width // 128)
-        self._store = like.new_empty(rows * chunks * 16 * bits + -(-rows // 128) * chunks * 512, dtype=torch.uint8)
         self._codes = self._scales = None
+        self._scales_at = at = rows * chunks * 16 * bits
+        self._store = like.new_empty(at + -(-rows // 128) * chunks * 512, dtype=torch.uint8)
         self.rows, self.width, self.bits, self.chunks, self.device_index = rows, width, bits, chunks, like.get_device()
         return self
 
     def _split(self) -> None:
-        row_bytes = self.chunks * 16 * self.bits
-        self._codes = self._store[: self.rows * row_bytes].view(self.rows, row_bytes)
-        self._scales = self._store[self.rows * row_bytes :].view(-(-self.rows // 128), self.chunks, 512)
+        self._codes = self._store[: self._scales_at].view(self.rows, self.chunks * 16 * self.bits)
+        self._scales = self._store[self._scales_at :].view(-(-self.rows // 128), self.chunks, 512)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -2605,9 +2605,10 @@ class Microscaled:
         """Of codes and scales, for a launch on the current device's stream."""
         if self.device_index != _current_device():
             raise KernelError(f"{what}: rows on device {self.device_index}, the current device is {_current_device()}")
-        if self._store is not None:
-            address = self._store.data_ptr()
-            return address, address + self.rows * self.chunks * 16 * self.bits
+        store = self._store
+        if store is not None:
+            address = store.data_ptr()
+            return address, address + self._scales_at
         return self._codes.data_ptr(), self._scales.data_ptr()
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -2624,11 +2625,11 @@ MICROSCALED_BITS = (4, 8)
 MICROSCALED_NORM_LARGEST_WIDTH = 32768
 
 
-def _check_here(what: str, *tensors: torch.Tensor) -> None:
+def _check_here(what: str, *tensors: "torch.Tensor | None") -> None:
     """Refuses tensors that do not lie on the current device, on whose stream the kernel is launched."""
     device = _current_device()
     for tensor in tensors:
-        if tensor.get_device() != device:
+        if tensor is not None and tensor.get_device() != device:
             raise KernelError(f"{what}: a tensor lies on device {tensor.get_device()}, the current device is {device}")
 
 
@@ -2660,38 +2661,37 @@ def rmsnorm_microscaled(x: torch.Tensor, weight: torch.Tensor, eps: float, *, de
         raise KernelError(f"rmsnorm_microscaled: elements have 4 or 8 bits, not {bits}")
     _check(x, "x", torch.float32)
     _check(weight, "weight", torch.float32)
-    if x.dim() != 2 or not 1 <= x.shape[1] <= MICROSCALED_NORM_LARGEST_WIDTH:
-        raise KernelError(f"rmsnorm_microscaled: x must be [rows, width] with a width of 1 to {MICROSCALED_NORM_LARGEST_WIDTH}, got {tuple(x.shape)}")
-    rows, width = x.shape
-    if weight.dim() != 1 or weight.shape[0] != width:
+    shape = x.shape
+    if len(shape) != 2 or not 1 <= shape[1] <= MICROSCALED_NORM_LARGEST_WIDTH:
+        raise KernelError(f"rmsnorm_microscaled: x must be [rows, width] with a width of 1 to {MICROSCALED_NORM_LARGEST_WIDTH}, got {tuple(shape)}")
+    rows, width = shape
+    if weight.shape != (width,):
         raise KernelError("rmsnorm_microscaled: weight must have one element per column")
-    here = [x, weight]
     code = 0
     if delta is not None:
         _check(delta, "delta")
-        if delta.shape != x.shape:
+        if delta.shape != shape:
             raise KernelError("rmsnorm_microscaled: delta and x differ in shape")
         code = dtype_code(delta.dtype)
-        here.append(delta)
     if sum_out is not None:
         _check(sum_out, "sum_out", torch.float32)
-        if sum_out.shape != x.shape:
+        if sum_out.shape != shape:
             raise KernelError("rmsnorm_microscaled: sum_out and x differ in shape")
-        if sum_out.data_ptr() != x.data_ptr() and _overlap(sum_out, x) or delta is not None and _overlap(sum_out, delta) or _overlap(sum_out, weight):
+        # between two addresses: the bytes from the lower one on that may not reach the other
+        size, own = 4 * rows * width, sum_out.data_ptr()
+        other, scale = own - x.data_ptr(), own - weight.data_ptr()
+        shares = -size < other < size and other != 0 or -size < scale < 4 * width
+        if delta is not None:
+            other = own - delta.data_ptr()
+            shares = shares or -size < other < delta.itemsize * rows * width
+        if shares and rows:
             raise KernelError("rmsnorm_microscaled: sum_out may be x, but not overlap it otherwise, nor delta or weight")
-        here.append(sum_out)
-    _check_here("rmsnorm_microscaled", *here)
+    _check_here("rmsnorm_microscaled", x, weight, delta, sum_out)
     out = Microscaled._empty(rows, width, bits, x)
     if rows:
         codes, scales = out._addresses("rmsnorm_microscaled")
         _done(_lib().lb_rmsnorm_microscaled(x, delta, sum_out, weight, scale_offset, eps, codes, scales, rows, width, bits, code, _stream()), "rmsnorm_microscaled")
     return out
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two contiguous tensors share bytes."""
-    first, second = a.data_ptr(), b.data_ptr()
-    return first < second + b.nbytes and second < first + a.nbytes
 
 
 def linear_microscaled(x: Microscaled, weight: Microscaled, out_dtype: torch.dtype = torch.bfloat16, status: torch.Tensor | None = None) -> torch.Tensor:
