@@ -72,6 +72,7 @@ def generate(
     max_batch_tokens: Annotated[int, Option(help="Tokens one step may run.")] = 2048,
     max_requests: Annotated[int, Option(help="Requests live at a time.")] = 64,
     chunk_size: Annotated[Optional[int], Option(help="Longest portion of one prompt in a step.", show_default="max-batch-tokens")] = None,
+    microscaled_feed_forward: Annotated[bool, Option("--microscaled-feed-forward", help="Hold the gated feed-forwards' weights in 4 bits (microscaled) and their rows in 8.")] = False,
     stats: Annotated[bool, Option(help="Print scheduler statistics to standard error.")] = False,
 ) -> None:
     from dataclasses import replace
@@ -99,7 +100,8 @@ def generate(
         prompts += [_parse_ids(line) for line in prompt_ids_file.read_text().splitlines() if line.strip()]
     if not prompts:
         _error("give --prompt-ids, --prompt-ids-file or --prompt")
-    engine_config = EngineConfig(dtype=dtype, page_size=page_size, max_tokens=max_cache_tokens, max_batch_tokens=max_batch_tokens, max_requests=max_requests)
+    engine_config = EngineConfig(dtype=dtype, page_size=page_size, max_tokens=max_cache_tokens, max_batch_tokens=max_batch_tokens, max_requests=max_requests,
+                                 microscaled_feed_forward=microscaled_feed_forward)
     try:
         if preset is not None or random_weights is not None:
             model = LanguageModel.random(preset if preset is not None else model_path, random_weights or 0, std=std, engine_config=engine_config, spec=spec)

@@ -539,9 +539,13 @@ struct MsSplit {
     static constexpr int kSlack = 1024 + 256;             // alignment and barriers
     static constexpr int kRoom = (kMsSplitShared - kSlack) / MsShape<BITS, BN>::kStageBytes;
     static constexpr int kMostStages = kRoom < kMsSplitStages ? kRoom : kMsSplitStages;
+    // A CTA waits for tensor memory without a limit, and one of a cluster keeps it until the others are done: clusters that wait for one another's would never
+    // end.  So a CTA takes at least that part of a multiprocessor's shared memory that it takes of its 512 columns, and what fits the one fits the other.
+    static constexpr int kLeast = kColumns * (kMsSharedLimit / 512) - 2048 < kMsSplitShared ? kColumns * (kMsSharedLimit / 512) - 2048 : kMsSplitShared;
+    static_assert(kColumns < 256 || kLeast + 2048 >= kMsSharedLimit / 2, "two CTAs of 256 columns leave no room for a third");
     static int bytes(int stages) {
-        const int ring = stages * MsShape<BITS, BN>::kStageBytes;
-        return (ring > kPartBytes ? ring : kPartBytes) + kSlack;
+        const int ring = stages * MsShape<BITS, BN>::kStageBytes, needed = (ring > kPartBytes ? ring : kPartBytes) + kSlack;
+        return needed > kLeast ? needed : kLeast;
     }
 };
 

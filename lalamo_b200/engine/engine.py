@@ -52,6 +52,7 @@ class EngineConfig:
     max_batch_tokens: int = 2048  # tokens one step may run (the scheduler's budget)
     device: str = "cuda:0"
     cuda_graphs: bool = True  # replay decode steps from CUDA graphs
+    microscaled_feed_forward: bool = False  # gated feed-forwards' weights in 4 bits with a scale per 32, their rows in 8 (bfloat16 engines)
     freeze_gc: bool = True  # after loading, exempt the objects alive so far from garbage collection passes
     poison_freed: bool = False  # tests: overwrite pages and state slots with NaN when they are given back
 
@@ -77,7 +78,7 @@ class Engine:
         self.engine_config = engine_config
         self.architecture_config = architecture_config
         self.plan = plan
-        self.runtime = Runtime(device=device, dtype=resolve_dtype(engine_config.dtype))
+        self.runtime = Runtime(device=device, dtype=resolve_dtype(engine_config.dtype), microscaled_feed_forward=engine_config.microscaled_feed_forward)
         self.model = DecoderModel(plan, tensors, self.runtime)
         page_size = engine_config.page_size
         self.cache = CacheManager(

@@ -3,6 +3,7 @@
     python -m lalamo_b200.microbench linear --tokens 512 --rows 2048 --width 8192 --epilogue residual_add [--tile 64]
     python -m lalamo_b200.microbench prefill-attention --tokens 2048 [--kernel mma] [--last-tiles 1]
     python -m lalamo_b200.microbench decode-attention --batch 8 --context 4096
+    python -m lalamo_b200.microbench microscaled --tokens 8 --rows 8192 --width 2048 --epilogue gated [--bits 4] --graph
     python -m lalamo_b200.microbench step-kernels --tokens 2048 [--preset lfm2-1.2b] [--batch 8 --context 4096]
 
 Each prints one JSON line.  Sizes default to the LFM2-1.2B shape (32 query heads over 8 K/V heads
@@ -73,6 +74,33 @@ def linear(arguments: argparse.Namespace) -> dict:
     microseconds = _time(run, arguments.repeats, arguments.graph) / len(weights)
     return {"kernel": "library" if arguments.library else "linear_tcgen05", "tokens": tokens, "rows": rows, "width": width, "epilogue": arguments.epilogue, "tile": arguments.tile or "auto",
             "slices": arguments.slices or "auto", "us": round(microseconds, 2), "tflops": round(2 * tokens * rows * width / microseconds / 1e6, 1)}
+
+
+def microscaled(arguments: argparse.Namespace) -> dict:
+    """Products of microscaled rows with weights of 4 bits, or with ``--epilogue quantise`` and ``norm`` what makes such rows."""
+    tokens, rows, width = arguments.tokens, arguments.rows, arguments.width
+    x = torch.randn(tokens, width, device="cuda")
+    if arguments.epilogue in ("quantise", "norm"):
+        half, weight, total = x.to(torch.bfloat16), torch.ones(width, device="cuda"), torch.empty_like(x)
+        run = (lambda: ops.microscale(half, arguments.bits)) if arguments.epilogue == "quantise" else (
+            lambda: ops.rmsnorm_microscaled(x, weight, 1e-5, delta=half, sum_out=total, bits=arguments.bits))
+        microseconds = _time(run, arguments.repeats, arguments.graph)
+        moved = tokens * width * ((2 if arguments.epilogue == "quantise" else 10) + arguments.bits / 8 + 1 / 32)
+        return {"kernel": arguments.epilogue, "tokens": tokens, "width": width, "bits": arguments.bits, "us": round(microseconds, 2), "gb_per_s": round(moved / microseconds / 1e3, 1)}
+    given = ops.microscale(x, arguments.bits)
+    weights = [[ops.microscale(torch.randn(rows, width, device="cuda") * 0.02, 4) for _ in range(2)] for _ in range(arguments.copies)]
+
+    def run_all() -> None:
+        for one, other in weights:
+            if arguments.epilogue == "gated":
+                ops.gated_linear_microscaled(given, one, other, "silu")
+            else:
+                ops.linear_microscaled(given, one, torch.float32 if arguments.epilogue == "store_float" else torch.bfloat16)
+
+    microseconds = _time(run_all, arguments.repeats, arguments.graph) / len(weights)
+    products = 2 if arguments.epilogue == "gated" else 1
+    return {"kernel": "microscaled product", "tokens": tokens, "rows": rows, "width": width, "bits": arguments.bits, "epilogue": arguments.epilogue, "us": round(microseconds, 2),
+            "tflops": round(2 * products * tokens * rows * width / microseconds / 1e6, 1), "weight_gb_per_s": round(products * rows * width * 17 / 32 / microseconds / 1e3, 1)}
 
 
 def prefill_attention(arguments: argparse.Namespace) -> dict:
@@ -199,6 +227,16 @@ def main(argv: list[str] | None = None) -> int:
     one.add_argument("--library", action="store_true", help="time torch.mm on the same shapes instead")
     one.add_argument("--auto", action="store_true", help="call the product the way the engine does (ops.linear, linear_accumulate, gated_linear)")
     one.set_defaults(function=linear)
+    one = commands.add_parser("microscaled")
+    one.add_argument("--tokens", type=int, default=2048)
+    one.add_argument("--rows", type=int, default=8192)
+    one.add_argument("--width", type=int, default=2048)
+    one.add_argument("--bits", type=int, default=8, choices=[8, 4], help="of the rows; weights have 4")
+    one.add_argument("--epilogue", default="store", choices=["store", "store_float", "gated", "quantise", "norm"])
+    one.add_argument("--copies", type=int, default=6)
+    one.add_argument("--repeats", type=int, default=20)
+    one.add_argument("--graph", action="store_true", help="record the loop in a CUDA graph and time its replays")
+    one.set_defaults(function=microscaled)
     for name, function in (("prefill-attention", prefill_attention), ("decode-attention", decode_attention)):
         one = commands.add_parser(name)
         one.add_argument("--heads", type=int, default=32)

@@ -71,11 +71,15 @@ class Runtime:
     device: torch.device
     dtype: torch.dtype  # activation / matrix type: torch.bfloat16 or torch.float32
     status: torch.Tensor = field(default=None)  # type: ignore[assignment]  # int32[1], first kernel error
+    # gated feed-forwards hold their weights in 4 bits and read rows of 8 (``ops.Microscaled``)
+    microscaled_feed_forward: bool = False
     _side_stream: "torch.cuda.Stream | None" = None
 
     def __post_init__(self) -> None:
         if self.dtype not in (torch.bfloat16, torch.float32):
             raise ValueError(f"the engine computes in bfloat16 or float32, not {self.dtype}")
+        if self.microscaled_feed_forward and self.dtype != torch.bfloat16:
+            raise ValueError(f"microscaled feed-forwards belong to a bfloat16 engine, not one of {self.dtype}")
         if self.status is None:
             self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
 
@@ -314,6 +318,9 @@ class FeedForward(Part):
     can_accumulate = False  # as for Mixer
     can_defer = False
     can_fork = False  # as for Mixer; and its first kernel is launched the ordinary way, behind everything it depends on
+    # True if forward() takes its input as ``ops.Microscaled`` rows of 8 bits as well: a norm in front of it then hands them out
+    # (``RMSNorm.residual_forward_microscaled``)
+    takes_microscaled = False
 
     def forward(self, x: torch.Tensor, step: StepInputs) -> torch.Tensor | None:
         raise NotImplementedError

@@ -112,6 +112,8 @@ class PreNormBlock(Block):
             mixed = self.mixer.forward(normed, step, cache)
         if self.ffn is None:
             return mixed   # the next block's norm (or the model's last) adds it
+        if self.ffn.takes_microscaled and hasattr(self.pre_ffn_norm, "residual_forward_microscaled"):
+            return self.ffn.forward(self.pre_ffn_norm.residual_forward_microscaled(residual, mixed), step)
         normed = self.pre_ffn_norm.residual_forward(residual, mixed)
         if self.ffn.can_accumulate:
             return self.ffn.forward(normed, step, residual=residual)

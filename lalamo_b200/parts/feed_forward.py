@@ -1,5 +1,7 @@
 """Dense gated feed-forward (``lalamo/modules/mlp.py:233-262``): ``down(up(x) * act(gate(x)))``
-with the up and gate projections fused into one product, rows ordered ``[up ; gate]``."""
+with the up and gate projections fused into one product, rows ordered ``[up ; gate]``.  Where the engine
+asks for it (``Runtime.microscaled_feed_forward``) the gated one holds its weights in 4 bits and reads and hands on rows of 8
+(``ops.Microscaled``)."""
 
 from __future__ import annotations
 
@@ -18,6 +20,10 @@ __all__ = ["DenseMLP", "GatedMLP"]
 class GatedMLP(FeedForward):
     def __init__(self, spec: GatedMLPSpec, tensors: Mapping[str, torch.Tensor], runtime: Runtime) -> None:
         super().__init__(spec, tensors, runtime)
+        self.takes_microscaled = runtime.microscaled_feed_forward
+        if self.takes_microscaled:
+            self.up, self.gate, self.down_rows = (ops.microscale(runtime.matrix(tensors[name]), 4) for name in ("up_proj", "gate_proj", "down_proj"))
+            return
         self.up_gate = runtime.matrix(torch.cat([tensors["up_proj"], tensors["gate_proj"]], dim=0))
         self.down = runtime.matrix(tensors["down_proj"])
 
@@ -32,7 +38,12 @@ class GatedMLP(FeedForward):
     can_accumulate = True
     can_defer = True
 
-    def forward(self, x: torch.Tensor, step: StepInputs | None = None, residual: torch.Tensor | None = None, defer: bool = False) -> "torch.Tensor | ops.SlicedSum | None":
+    def forward(self, x: "torch.Tensor | ops.Microscaled", step: StepInputs | None = None, residual: torch.Tensor | None = None,
+                defer: bool = False) -> "torch.Tensor | ops.SlicedSum | None":
+        if self.takes_microscaled:
+            rows = x if isinstance(x, ops.Microscaled) else ops.microscale(x, 8)
+            hidden = ops.gated_linear_microscaled(rows, self.up, self.gate, self.spec.activation, limit=self.spec.limit, status=self.runtime.status)
+            return ops.linear_microscaled(hidden, self.down_rows, self.runtime.dtype, status=self.runtime.status)   # the next norm adds it
         if x.shape[0] <= ops.SKINNY_MAX_TOKENS:
             out = ops.gated_mlp_step(x, self.up_gate, self.down, self.spec.activation, self.spec.limit, residual)
             if out is not None:

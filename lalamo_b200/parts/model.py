@@ -105,6 +105,8 @@ class DecoderModel:
                 if isinstance(value, torch.Tensor):
                     if value.is_cuda and value.data_ptr() != self.runtime.status.data_ptr():
                         seen[value.data_ptr()] = value.numel() * value.element_size()
+                elif isinstance(value, ops.Microscaled):
+                    seen[value.codes.data_ptr()] = value.codes.numel() + value.scales.numel()
                 elif isinstance(value, (Part, Block)) and depth < 4:
                     visit(value, depth + 1)
                 elif isinstance(value, list) and depth < 4:

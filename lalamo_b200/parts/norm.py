@@ -61,6 +61,13 @@ class RMSNorm(Norm):
         )
         return out
 
+    def residual_forward_microscaled(self, residual: torch.Tensor, delta: "torch.Tensor | ops.SlicedSum | ops.TermSum | None") -> "ops.Microscaled":
+        """As :meth:`residual_forward`, into rows of 8 bits with scales: 32-bit until the one rounding to them, also where the norm is not exact."""
+        if delta is not None and not isinstance(delta, torch.Tensor):
+            ops.residual_add(residual, delta)
+            delta = None
+        return ops.rmsnorm_microscaled(residual, self.scale, self.spec.eps, delta=delta, sum_out=None if delta is None else residual, scale_offset=self.spec.scale_offset)
+
     def streams_forward(self, streams: "ops.ResidualStreams", update: "ops.StreamWrite | None", read: torch.Tensor, *, keep: bool = True,
                         rows: torch.Tensor | None = None, num_rows: int | None = None, conv: dict | None = None) -> torch.Tensor:
         """On parallel residual streams: ``update`` written into them, then the norm of ``sum_s read[s] X_s``, one kernel
