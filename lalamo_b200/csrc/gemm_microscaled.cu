@@ -117,20 +117,6 @@ __device__ __forceinline__ uint32_t product_scales(int k) {
     return (byte << 4) | (byte << 29);
 }
 
-// What the gate side of a gated product multiplies with, and the up side.
-__device__ __forceinline__ float ms_gate_side(float g, int activation, float limit) {
-    if (activation == kSigmoidLimit) {
-        const float c = fminf(g, limit);
-        return __fdividef(c, 1.0f + __expf(-kSigmoidLimitSlope * c));
-    }
-    if (activation == 0) return __fdividef(g, 1.0f + __expf(-g));
-    if (activation == 1) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752440f));
-    return g;
-}
-__device__ __forceinline__ float ms_up_side(float u, int activation, float limit) {
-    return activation == kSigmoidLimit ? fminf(fmaxf(u, -limit), limit) + 1.0f : u;
-}
-
 // BN: tokens of a tile, of which a CTA loads OWN.  A tile of more than 128 begins at a multiple of 64, so that two tiles of scales cover it.
 template <int BITS, int BN, int OWN = BN>
 struct MsShape {
@@ -437,10 +423,10 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                     for (int b = 0; b < 2; ++b) {
                         const float* from = turned + token_here * kMsTurnedPitch + b * 32 + part * 4;
                         const float4 u = *reinterpret_cast<const float4*>(from), g = *reinterpret_cast<const float4*>(from + kMsRows / 2);
-                        h[b][0] = ms_up_side(u.x, p.activation, p.limit) * ms_gate_side(g.x, p.activation, p.limit);
-                        h[b][1] = ms_up_side(u.y, p.activation, p.limit) * ms_gate_side(g.y, p.activation, p.limit);
-                        h[b][2] = ms_up_side(u.z, p.activation, p.limit) * ms_gate_side(g.z, p.activation, p.limit);
-                        h[b][3] = ms_up_side(u.w, p.activation, p.limit) * ms_gate_side(g.w, p.activation, p.limit);
+                        h[b][0] = gated_up_side(u.x, p.activation, p.limit) * gated_gate_side(g.x, p.activation, p.limit);
+                        h[b][1] = gated_up_side(u.y, p.activation, p.limit) * gated_gate_side(g.y, p.activation, p.limit);
+                        h[b][2] = gated_up_side(u.z, p.activation, p.limit) * gated_gate_side(g.z, p.activation, p.limit);
+                        h[b][3] = gated_up_side(u.w, p.activation, p.limit) * gated_gate_side(g.w, p.activation, p.limit);
                         if (row0 + kMsRows / 2 > p.n) {   // past the last row: zeros, whatever the scales there
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
@@ -691,7 +677,9 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncwarp();
-    cluster_sync();   // all parts are there, or some CTA has failed and says so below
+    // all parts are there, or some CTA has failed and says so below
+    if (splits > 1) cluster_sync();
+    else __syncthreads();
     const int tokens_here = min(BN, p.tokens - token0);
     const uint32_t part = smem_address(ring);
     // Four rows (of a token) at each of two places, part after part; all parts are read before the first is added.
@@ -714,6 +702,9 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
                 sums[1].x += w[q].x, sums[1].y += w[q].y, sums[1].z += w[q].z, sums[1].w += w[q].w;
             }
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)   // here the sums exist, whether or not they are written: no read is under way any more
+            asm volatile("" ::"f"(sums[i].x), "f"(sums[i].y), "f"(sums[i].z), "f"(sums[i].w));
     };
     if constexpr (!GATED) {
         // A warp takes two tokens at a time, a lane four rows of each.
@@ -760,7 +751,7 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
             float h[4], largest = 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                h[e] = row0 + channel + e < p.n ? ms_up_side(up[e], p.activation, p.limit) * ms_gate_side(gate[e], p.activation, p.limit) : 0.0f;
+                h[e] = row0 + channel + e < p.n ? gated_up_side(up[e], p.activation, p.limit) * gated_gate_side(gate[e], p.activation, p.limit) : 0.0f;
                 largest = larger_size(largest, h[e]);
             }
 #pragma unroll
@@ -781,7 +772,9 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
         for (int spin = 0; spin < 2000; ++spin) __nanosleep(1000);
         __syncthreads();
     }
-    cluster_sync();   // nobody leaves while another still reads its part
+    // Nobody leaves while another still reads its part.  Nothing is to be ordered by it: what has been read is in registers (add_up sees to it), the output is of no
+    // concern to the others, and an arrival that waited for its writes would take some 800 cycles more.
+    if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Split::kColumns) : "memory");
 }
 

@@ -119,6 +119,20 @@ __device__ __forceinline__ uint32_t quantise_eight(const float (&v)[8], uint2& c
     return word;
 }
 
+// What the gate side of a gated product multiplies with, and the up side.
+__device__ __forceinline__ float gated_gate_side(float g, int activation, float limit) {
+    if (activation == kSigmoidLimit) {
+        const float c = fminf(g, limit);
+        return __fdividef(c, 1.0f + __expf(-kSigmoidLimitSlope * c));
+    }
+    if (activation == 0) return __fdividef(g, 1.0f + __expf(-g));
+    if (activation == 1) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752440f));
+    return g;
+}
+__device__ __forceinline__ float gated_up_side(float u, int activation, float limit) {
+    return activation == kSigmoidLimit ? fminf(fmaxf(u, -limit), limit) + 1.0f : u;
+}
+
 // Eight columns from `first` of a row of `width`, as float32; past the width zeros.  VECTOR: the row starts on 16 bytes and the width is a multiple of 8.
 template <bool VECTOR, typename T>
 __device__ __forceinline__ void load_eight(const T* row, int first, int width, float (&v)[8]) {
