@@ -28,7 +28,7 @@ struct MsParams {
     int out_is_float, bulk_store;
     int activation;
     float limit;
-    int row_tiles, token_tiles;
+    int row_tiles, token_tiles, wide_tiles;   // of the tokens' tiles the first wide_tiles have kMsWide, the others kMsNarrow
     int* status;
 };
 
@@ -160,6 +160,7 @@ __device__ __forceinline__ void issue_stage(uint32_t tmem_d, const unsigned char
     else mma_commit(empty);
 }
 
+constexpr int kMsWide = 192, kMsNarrow = 128;   // tokens of the walking kernel's tiles, which begin at multiples of 64
 constexpr int kMsThreads = 20 * 32;             // producer, issuer, scales of a gated product, one idle; sixteen warps of the epilogue
 constexpr int kMsGroup = 16;                    // tokens that four warps of the epilogue take at a time
 constexpr int kMsTurnedPitch = kMsRows + 4;     // floats: the 16 bytes of eight lanes and of the next token's lie in different banks
@@ -168,30 +169,31 @@ constexpr int kMsRegionBytes = 11 * 1024;       // per four warps: gated, 16 tok
 static_assert(kMsRegionBytes >= kMsTurnedBytes + 2 * kMsGroup * 64 && kMsRegionBytes >= kMsGroup * kMsRows * 4, "room for either");
 constexpr int kMsSharedLimit = 227 * 1024;
 
-template <int BITS, int BN, bool PAIR>
+template <int BITS, bool PAIR>
 struct MsWalk {
+    static constexpr int BN = kMsWide;
     using Shape = MsShape<BITS, BN, PAIR ? BN / 2 : BN>;
     static constexpr int kStages = (kMsSharedLimit - 4 * kMsRegionBytes - 1024 - 256) / Shape::kStageBytes;
     static constexpr int kBytes = kStages * Shape::kStageBytes + 4 * kMsRegionBytes + 1024 + 256;
     static constexpr int kScaleSet = 4 * Shape::kChunks * (1 + Shape::kScaleTiles);
     static constexpr int kScaleColumns = (PAIR ? 2 : 1) * kScaleSet;
-    static constexpr int kColumns = 2 * BN + kScaleColumns <= 256 ? 256 : 512;
-    static_assert(kStages >= 3 && kStages <= 12 && 2 * BN + kScaleColumns <= 512, "a ring, its barriers, two accumulators and the scales");
+    static constexpr int kColumns = 512;
+    static_assert(kStages >= 3 && kStages <= 12 && 2 * BN + kScaleColumns <= kColumns, "a ring, its barriers, two accumulators and the scales");
 };
 
-// One CTA per multiprocessor walks the tiles of 128 lanes x BN tokens, rows fastest, with two accumulators: the epilogue of a tile runs while the
+// One CTA per multiprocessor walks the tiles of 128 lanes x 192 or 128 tokens, rows fastest, with two accumulators: the epilogue of a tile runs while the
 // products of the next are issued.  PAIR: the walkers are pairs of CTAs that share a tile of 256 lanes; each loads its rows of W, half of the tokens and all
 // of their scales, all bytes count on the even CTA's barriers, and that one issues products over both CTAs' shared and tensor memory.  (Not for gated products,
 // whose scales would have to be announced across the pair, nor rows of 4 bits: 4096 x 8192 x 2048 40.3 us and 38.0 without.)
-template <int BITS, int BN, bool GATED, bool PAIR>
+template <int BITS, bool GATED, bool PAIR>
 __global__ void __launch_bounds__(kMsThreads)
 gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_gate, const __grid_constant__ CUtensorMap map_x,
-                        const __grid_constant__ CUtensorMap map_w_scales, const __grid_constant__ CUtensorMap map_x_scales, const __grid_constant__ CUtensorMap map_out,
+                        const __grid_constant__ CUtensorMap map_x_narrow, const __grid_constant__ CUtensorMap map_w_scales, const __grid_constant__ CUtensorMap map_x_scales, const __grid_constant__ CUtensorMap map_out,
                         const MsParams p) {
     static_assert(!PAIR || (BITS == 8 && !GATED), "what pairs take");
-    using Walk = MsWalk<BITS, BN, PAIR>;
+    using Walk = MsWalk<BITS, PAIR>;
     using Shape = typename Walk::Shape;
-    constexpr int STAGES = Walk::kStages;
+    constexpr int STAGES = Walk::kStages, BN = Walk::BN;
     constexpr int kPairs = PAIR ? 2 : 1;   // CTAs of a walker
     const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
     const int walker = static_cast<int>(blockIdx.x) / kPairs, walkers = static_cast<int>(gridDim.x) / kPairs;
@@ -212,7 +214,13 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     const int num_tiles = p.row_tiles * p.token_tiles;
     auto chunks_of = [&](int stage) { return min(Shape::kChunks, p.chunks - stage * Shape::kChunks); };
     auto row_of = [&](int tile) { return ((tile % p.row_tiles) * kPairs + rank) * kRowsPerCta; };   // this CTA's first
-    auto token_of = [&](int tile) { return tile / p.row_tiles * BN; };
+    auto is_wide = [&](int tile) { return tile / p.row_tiles < p.wide_tiles; };
+    auto token_of = [&](int tile) {
+        const int index = tile / p.row_tiles;
+        return index * kMsNarrow + min(index, p.wide_tiles) * (kMsWide - kMsNarrow);
+    };
+    // The tokens that a tile's products take: the last tile's only as many as there are, in whole 16s of each CTA.
+    auto columns_of = [&](int tile) { return min(is_wide(tile) ? kMsWide : kMsNarrow, (p.tokens - token_of(tile) + 16 * kPairs - 1) / (16 * kPairs) * (16 * kPairs)); };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -249,7 +257,9 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         int s = 0, round = 0;
         bool ok = true;
         for (int tile = walker; tile < num_tiles && ok; tile += walkers) {
-            const int row0 = row_of(tile), token0 = token_of(tile);
+            const int row0 = row_of(tile), token0 = token_of(tile), own_token0 = token0 + rank * (columns_of(tile) / 2);
+            const bool wide = is_wide(tile);
+            const uint32_t x_bytes = static_cast<uint32_t>((wide ? kMsWide : kMsNarrow) / kPairs * 128);
             for (int stage = 0; stage < num_stages; ++stage) {
                 ok = round == 0 || barrier_wait_warp<PAIR>(&empty[s], (round - 1) & 1);
                 if (!ok) {
@@ -260,14 +270,14 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                     unsigned char* at = ring + s * Shape::kStageBytes;
                     const int column = stage * 128;   // of the map: elements of W where they are spread and of X in 8 bits, bytes of rows in 4
                     const int word = stage * Shape::kChunks * (kScaleTileBytes / 4);
-                    if (rank == 0) barrier_expect(&full[s], kPairs * (Shape::kWCounted + Shape::kXBytes + (GATED ? 0 : Shape::kWScaleBytes) + Shape::kXScaleBytes));
+                    if (rank == 0) barrier_expect(&full[s], kPairs * (Shape::kWCounted + x_bytes + (GATED ? 0 : Shape::kWScaleBytes) + Shape::kXScaleBytes));
                     auto load = [&](void* to, const CUtensorMap* map, int x, int y) {
                         if constexpr (PAIR) tma_load_2d_pair(to, map, x, y, cluster_address(&full[s], 0));
                         else tma_load_2d(to, map, x, y, &full[s]);
                     };
                     load(at, &map_w, column, row0);
                     if constexpr (GATED) load(at + Shape::kWBytes / 2, &map_gate, column, row0);
-                    load(at + Shape::kWBytes, &map_x, column, token0 + rank * (BN / 2));
+                    load(at + Shape::kWBytes, wide ? &map_x : &map_x_narrow, column, own_token0);
                     at += Shape::kWBytes + Shape::kXBytes;
                     if constexpr (!GATED) load(at, &map_w_scales, word, row0 / 128);
                     load(at + Shape::kWScaleBytes, &map_x_scales, word, token0 / 128);
@@ -276,7 +286,6 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
             }
         }
     } else if (warp == 1) {
-        const uint32_t idesc = microscaled_descriptor<BITS>(BN, kPairs * kMsRows);
         int s = 0, round = 0, local = 0, left = (num_tiles - walker + walkers - 1) / walkers * num_stages;
         uint32_t set = 0u;
         bool ok = rank == 0, copied = false;
@@ -285,6 +294,7 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
             ok = use == 0 || barrier_wait_warp<PAIR>(&tmem_empty[accumulator], (use - 1) & 1);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(accumulator * BN);
+            const uint32_t idesc = microscaled_descriptor<BITS>(columns_of(tile), kPairs * kMsRows);
             const uint32_t token_column = static_cast<uint32_t>((token_of(tile) & 127) >> 5);   // of the scales: 32 tokens a column
             for (int stage = 0; stage < num_stages && ok; ++stage) {
                 const unsigned char* at = ring + s * Shape::kStageBytes;
@@ -402,7 +412,7 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(accumulator * BN) + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-            for (int column = set * kMsGroup; column < BN; column += 4 * kMsGroup, ++groups) {
+            for (int column = set * kMsGroup; column < (is_wide(tile) ? kMsWide : kMsNarrow); column += 4 * kMsGroup, ++groups) {
                 const int first_token = token0 + column;
                 if (first_token >= p.tokens) break;   // the same for the whole set
                 uint32_t v[kMsGroup];
@@ -816,13 +826,15 @@ static bool make_scales_map(CUtensorMap* map, const void* scales, int row_tiles,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BITS, int BN, bool GATED, bool PAIR>
-int launch_microscaled(const void* x, const void* w, const void* gate, MsParams p, cudaStream_t stream) {
-    using Walk = MsWalk<BITS, BN, PAIR>;
+template <int BITS, bool GATED, bool PAIR>
+int launch_microscaled(const void* x, const void* w, const void* gate, MsParams p, int token_tiles, int wide_tiles, cudaStream_t stream) {
+    using Walk = MsWalk<BITS, PAIR>;
     using Shape = typename Walk::Shape;
-    CUtensorMap map_w, map_gate, map_x, map_w_scales, map_x_scales, map_out;
+    constexpr int kCtas = PAIR ? 2 : 1;
+    CUtensorMap map_w, map_gate, map_x, map_x_narrow, map_w_scales, map_x_scales, map_out;
     const int w_bytes = p.chunks * 64, x_bytes = p.chunks * 16 * BITS;
-    if (!make_codes_map(&map_w, w, p.n, w_bytes, GATED ? kMsRows / 2 : kMsRows, BITS == 8) || !make_codes_map(&map_x, x, p.tokens, x_bytes, PAIR ? BN / 2 : BN, false) ||
+    if (!make_codes_map(&map_w, w, p.n, w_bytes, GATED ? kMsRows / 2 : kMsRows, BITS == 8) || !make_codes_map(&map_x, x, p.tokens, x_bytes, kMsWide / kCtas, false) ||
+        !make_codes_map(&map_x_narrow, x, p.tokens, x_bytes, kMsNarrow / kCtas, false) ||
         !make_scales_map(&map_w_scales, p.w_scales, (p.n + 127) / 128, p.chunks, 1, Shape::kChunks) ||
         !make_scales_map(&map_x_scales, p.x_scales, (p.tokens + 127) / 128, p.chunks, Shape::kScaleTiles, Shape::kChunks))
         return -5;
@@ -841,14 +853,15 @@ int launch_microscaled(const void* x, const void* w, const void* gate, MsParams 
             return -5;
         row_tiles = (p.n + kMsRows - 1) / kMsRows;
     }
-    p.row_tiles = PAIR ? (row_tiles + 1) / 2 : row_tiles;
-    p.token_tiles = (p.tokens + BN - 1) / BN;
-    auto kernel = gemm_microscaled_kernel<BITS, BN, GATED, PAIR>;
+    p.row_tiles = (row_tiles + kCtas - 1) / kCtas;
+    p.token_tiles = token_tiles;
+    p.wide_tiles = wide_tiles;
+    auto kernel = gemm_microscaled_kernel<BITS, GATED, PAIR>;
     static OncePerDevice configured;
     if (allow_shared_memory(configured, kernel, Walk::kBytes) != cudaSuccess) return static_cast<int>(cudaGetLastError());
-    const int tiles = p.row_tiles * p.token_tiles, walkers = multiprocessor_count() / (PAIR ? 2 : 1);
+    const int tiles = p.row_tiles * p.token_tiles, walkers = multiprocessor_count() / kCtas;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((tiles < walkers ? tiles : walkers) * (PAIR ? 2 : 1));
+    config.gridDim = dim3((tiles < walkers ? tiles : walkers) * kCtas);
     config.blockDim = dim3(kMsThreads);
     config.dynamicSmemBytes = Walk::kBytes;
     config.stream = stream;
@@ -861,7 +874,7 @@ int launch_microscaled(const void* x, const void* w, const void* gate, MsParams 
     attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = PAIR ? 2 : 1;
-    return static_cast<int>(cudaLaunchKernelEx(&config, kernel, map_w, map_gate, map_x, map_w_scales, map_x_scales, map_out, p));
+    return static_cast<int>(cudaLaunchKernelEx(&config, kernel, map_w, map_gate, map_x, map_x_narrow, map_w_scales, map_x_scales, map_out, p));
 }
 
 template <int BITS, int BN, bool GATED>
@@ -903,27 +916,44 @@ int launch_microscaled_split(const void* x, const void* w, const void* gate, MsP
     return static_cast<int>(cudaLaunchKernelEx(&config, kernel, map_w, map_gate, map_x, p, splits, per_split, ring));
 }
 
-// Which kernel.  Few tiles are cut along K: up to 128 tokens, and up to half of the multiprocessors in tiles of 128 x 128.  Else the tiles are walked, and what decides is
-// how many rounds of tiles a walker has and what a stage of K costs in each (measured under sustained load at 4,096 tokens, 2048 x 8192: 0.29 us with 128 tokens a
-// tile, 0.36 with 192, 0.32 of a pair with 192), a pair some 2.5 us at the start.  With 2,048 tokens and 2048 x 2048 tiles of 128 tokens take 11.7 us,
-// of 192 13.1 and pairs 13.8; with 777 and 6912 x 1536 12.8, 11.7 and 11.1.
+// How the tokens are cut into tiles: of all numbers of tiles, the first as many of them wide as it takes, the one whose first walker, which has the most and the widest
+// tiles, is done first.  What a stage of K costs (hundredths of a microsecond, measured at 4,096 tokens, 2048 x 8192, under sustained load): 29 with 128 tokens and 36
+// with 192; of a pair 27 and 32; with rows of 4 bits 30 and 36.
+struct TokenTiles {
+    int count, wide;
+    long long cost;   // of the walk
+};
+inline TokenTiles cut_tokens(int tokens, long long row_tiles, int walkers, long long stages, int narrow_cost, int wide_cost) {
+    TokenTiles best = {0, 0, -1};
+    for (int count = (tokens + kMsWide - 1) / kMsWide; count <= (tokens + kMsNarrow - 1) / kMsNarrow; ++count) {
+        const int more = tokens - count * kMsNarrow, step = kMsWide - kMsNarrow, wide = more > 0 ? (more + step - 1) / step : 0;
+        const int last = tokens - ((count - 1) * kMsNarrow + min(wide, count - 1) * step);   // tokens of the last tile
+        // rounds of the first walker: all, those that begin before the last tile, and of these those with a wide tile
+        const auto rounds = [&](int tiles) { return (row_tiles * tiles + walkers - 1) / walkers; };
+        const long long before = rounds(count - 1), wides = min(rounds(min(wide, count - 1)), before);
+        const long long cost = wides * wide_cost + (before - wides) * narrow_cost + (rounds(count) - before) * (narrow_cost + (last - kMsNarrow) * (wide_cost - narrow_cost) / step);
+        if (best.cost < 0 || cost * stages < best.cost) best = {count, wide, cost * stages};
+    }
+    return best;
+}
+
+// Which kernel.  Few tiles are cut along K: up to 128 tokens, and up to half of the multiprocessors in tiles of 128 x 128.  Else the tiles are walked, by pairs of CTAs where
+// those are sooner done although they start some 2.5 us later.
 template <int BITS, bool GATED>
 int launch_microscaled_tiles(const void* x, const void* w, const void* gate, const MsParams& p, cudaStream_t stream) {
-    const long long row_tiles = GATED ? p.out_chunks * 2 : (p.n + kMsRows - 1) / kMsRows, narrow = row_tiles * ((p.tokens + 127) / 128);
+    const long long row_tiles = GATED ? p.out_chunks * 2 : (p.n + kMsRows - 1) / kMsRows;
     const int sms = multiprocessor_count();
     if (p.tokens <= 16) return launch_microscaled_split<BITS, 16, GATED>(x, w, gate, p, stream);
     if (p.tokens <= 32) return launch_microscaled_split<BITS, 32, GATED>(x, w, gate, p, stream);
     if (p.tokens <= 64) return launch_microscaled_split<BITS, 64, GATED>(x, w, gate, p, stream);
-    if (p.tokens <= 128 || narrow <= sms / 2) return launch_microscaled_split<BITS, 128, GATED>(x, w, gate, p, stream);
-    const int wide_tokens = (p.tokens + 191) / 192;
+    if (p.tokens <= 128 || row_tiles * ((p.tokens + 127) / 128) <= sms / 2) return launch_microscaled_split<BITS, 128, GATED>(x, w, gate, p, stream);
     const long long stages = (p.chunks + MsShape<BITS, 128>::kChunks - 1) / MsShape<BITS, 128>::kChunks;
-    const long long narrow_cost = (narrow + sms - 1) / sms * stages * 29, wide_cost = (row_tiles * wide_tokens + sms - 1) / sms * stages * 36;
+    const TokenTiles alone = cut_tokens(p.tokens, row_tiles, sms, stages, BITS == 8 ? 29 : 30, 36);
     if constexpr (BITS == 8 && !GATED) {
-        const long long pairs = sms / 2, pair_cost = ((row_tiles + 1) / 2 * wide_tokens + pairs - 1) / pairs * stages * 32 + 250;
-        if (pair_cost < narrow_cost && pair_cost < wide_cost) return launch_microscaled<BITS, 192, GATED, true>(x, w, gate, p, stream);
+        const TokenTiles pairs = cut_tokens(p.tokens, (row_tiles + 1) / 2, sms / 2, stages, 27, 32);
+        if (pairs.cost + 250 < alone.cost) return launch_microscaled<BITS, GATED, true>(x, w, gate, p, pairs.count, pairs.wide, stream);
     }
-    if (narrow_cost < wide_cost) return launch_microscaled<BITS, 128, GATED, false>(x, w, gate, p, stream);
-    return launch_microscaled<BITS, 192, GATED, false>(x, w, gate, p, stream);
+    return launch_microscaled<BITS, GATED, false>(x, w, gate, p, alone.count, alone.wide, stream);
 }
 
 }  // namespace lb
