@@ -5,7 +5,6 @@
 namespace lb {
 
 constexpr int kMicroscaleThreads = 256;
-constexpr int kMicroscaleUnroll = 4;   // pieces of 128 columns that sixteen lanes have in flight
 
 // Division of numbers below 2^31 by one that the host knows: with l = ceil(log2 d) and m = ceil(2^(31 + l) / d), n / d = n m >> (31 + l), exact for those n
 // (m d exceeds 2^(31 + l) by less than d <= 2^l).
@@ -19,41 +18,60 @@ inline Divisor divisor_of(unsigned d) {
     return {d, d == 1 ? 0u : static_cast<unsigned>(((1ull << (31 + l)) + d - 1) / d), l - 1};
 }
 
-// Pieces of 128 columns under one word of scales, `chunks` of them a row: sixteen lanes take one, eight columns each, and each group of sixteen
-// kMicroscaleUnroll of them.  (There are fewer than 2^31: the rows would not fit the GPU.)
+// Pieces of 128 columns under one word of scales, `chunks` of them a row, LANES lanes to each; a block takes ROUNDS rounds of them.  (There are fewer than
+// 2^31: the rows would not fit the GPU.)
 struct Piece {
     int row, chunk;
     bool exists;
 };
+template <int LANES, int ROUNDS>
 __device__ __forceinline__ Piece piece_of(int u, unsigned total, const Divisor& chunks) {
-    const unsigned piece = blockIdx.x * (kMicroscaleThreads / 16 * kMicroscaleUnroll) + u * (kMicroscaleThreads / 16) + (threadIdx.x >> 4);
+    const unsigned piece = (blockIdx.x * ROUNDS + u) * (kMicroscaleThreads / LANES) + threadIdx.x / LANES;
     const unsigned row = chunks.quotient(piece);
     return {static_cast<int>(row), static_cast<int>(piece - row * chunks.divisor), piece < total};
 }
+template <int LANES, int ROUNDS>
+dim3 microscale_grid(unsigned pieces) {
+    constexpr unsigned per_block = kMicroscaleThreads / LANES * ROUNDS;
+    return dim3((pieces + per_block - 1) / per_block);
+}
+
+// How many columns of x a lane takes at a time and how often, by the type.  Of bfloat16 sixteen, two loads of 16 bytes: what is done once a lane, places and scales, is
+// then half of what it is with eight, and instructions bound that (16,384 x 2,048 to 8 bits: 15.9 us, 6.4 TB/s, and 19.7 with eight).  Of float32, which memory bounds,
+// eight and once (25.7 us, 6.6 TB/s; four times 27.8).
+template <typename T>
+struct MicroscaleShape {
+    static constexpr int kCount = sizeof(T) == 2 ? 16 : 8, kLanes = 128 / kCount, kRounds = sizeof(T) == 2 ? 2 : 1;
+};
+// The same of the values' kernel: eight columns, four times of bfloat16 (14.9 us, 6.8 TB/s; once 19.9), once of float32 (32.0 us; four times 36.4).
+template <typename T>
+constexpr int kValuesRounds = sizeof(T) == 2 ? 4 : 1;
 
 // codes and scales of x [rows, width]
 template <typename T, int BITS, bool VECTOR>
 __global__ void __launch_bounds__(kMicroscaleThreads)
 microscale_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, int width, unsigned total, Divisor chunks) {
+    constexpr int kCount = MicroscaleShape<T>::kCount, kLanes = MicroscaleShape<T>::kLanes, kRounds = MicroscaleShape<T>::kRounds;
     wait_for_previous_kernel();
     allow_next_kernel();
-    const int column = (threadIdx.x & 15) * 8;
-    Piece piece[kMicroscaleUnroll];
-    float v[kMicroscaleUnroll][8];
+    const int column = threadIdx.x % kLanes * kCount;
+    Piece piece[kRounds];
+    float v[kRounds][kCount];
 #pragma unroll
-    for (int u = 0; u < kMicroscaleUnroll; ++u) {
-        piece[u] = piece_of(u, total, chunks);
+    for (int u = 0; u < kRounds; ++u) {
+        piece[u] = piece_of<kLanes, kRounds>(u, total, chunks);
         // a piece that does not exist counts as one past its row's width: zeros
-        load_eight<VECTOR>(x + static_cast<size_t>(piece[u].row) * width, piece[u].exists ? piece[u].chunk * 128 + column : width, width, v[u]);
+        const T* row = x + static_cast<size_t>(piece[u].row) * width;
+        const int first = piece[u].exists ? piece[u].chunk * 128 + column : width;
+        load_eight<VECTOR>(row, first, width, v[u]);
+        if constexpr (kCount == 16) load_eight<VECTOR, 8>(row, first + 8, width, v[u]);
     }
 #pragma unroll
-    for (int u = 0; u < kMicroscaleUnroll; ++u) {
-        uint2 code;
-        const uint32_t word = quantise_eight<BITS>(v[u], code);
+    for (int u = 0; u < kRounds; ++u) {
+        uint32_t code[kCount * BITS / 32];
+        const uint32_t word = quantise<BITS>(v[u], code);
         if (!piece[u].exists) continue;
-        const size_t at = (static_cast<size_t>(piece[u].row) * chunks.divisor + piece[u].chunk) * 128 + column;
-        if constexpr (BITS == 8) *reinterpret_cast<uint2*>(codes + at) = code;
-        else *reinterpret_cast<uint32_t*>(codes + at / 2) = code.x;
+        store_codes(codes + ((static_cast<size_t>(piece[u].row) * chunks.divisor + piece[u].chunk) * 128 + column) * BITS / 8, code);
         if (column == 0) *reinterpret_cast<uint32_t*>(scales + scale_word(piece[u].row, piece[u].chunk, chunks.divisor)) = word;
     }
 }
@@ -65,13 +83,14 @@ __global__ void __launch_bounds__(kMicroscaleThreads)
 microscaled_values_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales, T* __restrict__ out, int width, unsigned total, Divisor chunks) {
     wait_for_previous_kernel();
     allow_next_kernel();
+    constexpr int kRounds = kValuesRounds<T>;
     const int column = (threadIdx.x & 15) * 8;
-    Piece piece[kMicroscaleUnroll];
-    uint2 code[kMicroscaleUnroll];
-    int byte[kMicroscaleUnroll];
+    Piece piece[kRounds];
+    uint2 code[kRounds];
+    int byte[kRounds];
 #pragma unroll
-    for (int u = 0; u < kMicroscaleUnroll; ++u) {
-        piece[u] = piece_of(u, total, chunks);
+    for (int u = 0; u < kRounds; ++u) {
+        piece[u] = piece_of<16, kRounds>(u, total, chunks);
         if (!piece[u].exists) continue;
         const size_t at = (static_cast<size_t>(piece[u].row) * chunks.divisor + piece[u].chunk) * 128 + column;
         if constexpr (BITS == 8) code[u] = *reinterpret_cast<const uint2*>(codes + at);
@@ -79,7 +98,7 @@ microscaled_values_kernel(const unsigned char* __restrict__ codes, const unsigne
         byte[u] = scales[scale_word(piece[u].row, piece[u].chunk, chunks.divisor) + column / 32];
     }
 #pragma unroll
-    for (int u = 0; u < kMicroscaleUnroll; ++u) {
+    for (int u = 0; u < kRounds; ++u) {
         if (!piece[u].exists) continue;
         const float scale = scale_value(byte[u]);
         float v[8];
@@ -128,12 +147,10 @@ rmsnorm_microscaled_kernel(const float* x, const TD* __restrict__ delta, float* 
         load_eight<VECTOR>(weight, column, width, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = column + i < width ? v[g][i] * factor * (w[i] + offset) : 0.0f;
-        uint2 code;
-        const uint32_t word = quantise_eight<BITS>(w, code);
+        uint32_t code[BITS / 4];
+        const uint32_t word = quantise<BITS>(w, code);
         if (column >= chunks * 128) continue;
-        const size_t at = static_cast<size_t>(row) * chunks * 128 + column;
-        if constexpr (BITS == 8) *reinterpret_cast<uint2*>(codes + at) = code;
-        else *reinterpret_cast<uint32_t*>(codes + at / 2) = code.x;
+        store_codes(codes + (static_cast<size_t>(row) * chunks * 128 + column) * BITS / 8, code);
         if ((column & 127) == 0) *reinterpret_cast<uint32_t*>(scales + scale_word(row, column >> 7, chunks)) = word;
     }
 }
@@ -143,16 +160,11 @@ bool rows_are_aligned(const T* rows, int width) {
     return width % 8 == 0 && (reinterpret_cast<uintptr_t>(rows) & 15) == 0;
 }
 
-inline dim3 microscale_grid(unsigned pieces) {
-    constexpr unsigned per_block = kMicroscaleThreads / 16 * kMicroscaleUnroll;
-    return dim3((pieces + per_block - 1) / per_block);
-}
-
 template <typename T, int BITS>
 cudaError_t launch_microscale(const T* x, unsigned char* codes, unsigned char* scales, int rows, int width, cudaStream_t stream) {
     const int chunks = (width + 127) / 128;
     auto kernel = rows_are_aligned(x, width) ? microscale_kernel<T, BITS, true> : microscale_kernel<T, BITS, false>;
-    return launch_overlapped(kernel, microscale_grid(static_cast<unsigned>(rows) * chunks), dim3(kMicroscaleThreads), 0, stream, x, codes, scales, width,
+    return launch_overlapped(kernel, microscale_grid<MicroscaleShape<T>::kLanes, MicroscaleShape<T>::kRounds>(static_cast<unsigned>(rows) * chunks), dim3(kMicroscaleThreads), 0, stream, x, codes, scales, width,
                              static_cast<unsigned>(rows) * chunks, divisor_of(chunks));
 }
 
@@ -160,7 +172,7 @@ template <typename T, int BITS>
 cudaError_t launch_values(const unsigned char* codes, const unsigned char* scales, T* out, int rows, int width, cudaStream_t stream) {
     const int chunks = (width + 127) / 128;
     auto kernel = rows_are_aligned(out, width) ? microscaled_values_kernel<T, BITS, true> : microscaled_values_kernel<T, BITS, false>;
-    return launch_overlapped(kernel, microscale_grid(static_cast<unsigned>(rows) * chunks), dim3(kMicroscaleThreads), 0, stream, codes, scales, out, width,
+    return launch_overlapped(kernel, microscale_grid<16, kValuesRounds<T>>(static_cast<unsigned>(rows) * chunks), dim3(kMicroscaleThreads), 0, stream, codes, scales, out, width,
                              static_cast<unsigned>(rows) * chunks, divisor_of(chunks));
 }
 

@@ -58,7 +58,7 @@ __device__ __forceinline__ uint32_t pack_e2m1(const float (&v)[8]) {
     return packed;
 }
 
-// The elements of eight consecutive columns, without their scale: what quantise_eight packs.
+// The elements of eight consecutive columns, without their scale.
 template <int BITS>
 __device__ __forceinline__ void unpack_eight(uint2 codes, float (&v)[8]) {
     uint32_t pairs[4];   // float16, which holds every element of both formats
@@ -93,30 +93,43 @@ __device__ __forceinline__ float larger_size(float a, float b) {
     return c;
 }
 
-// Quantises eight consecutive columns a lane: four lanes hold a block, sixteen the 128 columns under one word of scales.  All lanes of the warp take part.
-// Returns that word (the same in the sixteen lanes); `codes` has eight bytes, or four bytes of halves in codes.x.  (What the elements of a block
-// are that has no number for a scale says nothing.)
-template <int BITS>
-__device__ __forceinline__ uint32_t quantise_eight(const float (&v)[8], uint2& codes) {
-    float largest = larger_size(larger_size(larger_size(v[0], v[1]), larger_size(v[2], v[3])), larger_size(larger_size(v[4], v[5]), larger_size(v[6], v[7])));
-    largest = larger_size(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-    largest = larger_size(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+// Quantises eight or sixteen consecutive columns a lane: four (two) lanes hold a block, sixteen (eight) the 128 columns under one word of scales.  All lanes of
+// the warp take part.  Returns that word (the same in all of them); `codes` has four bytes, or two bytes of halves, for every four columns.  (What the
+// elements of a block are that has no number for a scale says nothing.)
+template <int BITS, int COUNT>
+__device__ __forceinline__ uint32_t quantise(const float (&v)[COUNT], uint32_t (&codes)[COUNT * BITS / 32]) {
+    constexpr int kLanes = 32 / COUNT;   // of a block
+    float largest = larger_size(v[0], v[1]);
+#pragma unroll
+    for (int i = 2; i < COUNT; i += 2) largest = larger_size(largest, larger_size(v[i], v[i + 1]));
+#pragma unroll
+    for (int offset = 1; offset < kLanes; offset <<= 1) largest = larger_size(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
     const int byte = scale_byte<BITS>(__float_as_uint(largest) & 0x7fffffffu);
     const float inverse = scale_inverse(byte);
-    float scaled[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) scaled[i] = v[i] * inverse;
     if constexpr (BITS == 8) {
-        codes.x = pack_e4m3(scaled[0], scaled[1], scaled[2], scaled[3]);
-        codes.y = pack_e4m3(scaled[4], scaled[5], scaled[6], scaled[7]);
+#pragma unroll
+        for (int i = 0; i < COUNT / 4; ++i) codes[i] = pack_e4m3(v[4 * i] * inverse, v[4 * i + 1] * inverse, v[4 * i + 2] * inverse, v[4 * i + 3] * inverse);
     } else {
-        codes.x = pack_e2m1(scaled);
-        codes.y = 0u;
+#pragma unroll
+        for (int i = 0; i < COUNT / 8; ++i) {
+            float scaled[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) scaled[e] = v[8 * i + e] * inverse;
+            codes[i] = pack_e2m1(scaled);
+        }
     }
-    uint32_t word = static_cast<uint32_t>(byte) << (((threadIdx.x >> 2) & 3) * 8);
-    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    uint32_t word = static_cast<uint32_t>(byte) << ((threadIdx.x / kLanes & 3) * 8);
+    word |= __shfl_xor_sync(0xffffffffu, word, kLanes);
+    word |= __shfl_xor_sync(0xffffffffu, word, 2 * kLanes);
     return word;
+}
+
+// Its codes, at a place that their bytes divide.
+template <int WORDS>
+__device__ __forceinline__ void store_codes(unsigned char* to, const uint32_t (&codes)[WORDS]) {
+    if constexpr (WORDS == 4) *reinterpret_cast<uint4*>(to) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+    else if constexpr (WORDS == 2) *reinterpret_cast<uint2*>(to) = make_uint2(codes[0], codes[1]);
+    else *reinterpret_cast<uint32_t*>(to) = codes[0];
 }
 
 // What the gate side of a gated product multiplies with, and the up side.
@@ -133,28 +146,28 @@ __device__ __forceinline__ float gated_up_side(float u, int activation, float li
     return activation == kSigmoidLimit ? fminf(fmaxf(u, -limit), limit) + 1.0f : u;
 }
 
-// Eight columns from `first` of a row of `width`, as float32; past the width zeros.  VECTOR: the row starts on 16 bytes and the width is a multiple of 8.
-template <bool VECTOR, typename T>
-__device__ __forceinline__ void load_eight(const T* row, int first, int width, float (&v)[8]) {
+// Eight columns from `first` of a row of `width`, as float32, into v[at] on; past the width zeros.  VECTOR: the row starts on 16 bytes and the width is a multiple of 8.
+template <bool VECTOR, int at = 0, typename T, int COUNT>
+__device__ __forceinline__ void load_eight(const T* row, int first, int width, float (&v)[COUNT]) {
     if constexpr (VECTOR) {
         if (first >= width) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+            for (int i = 0; i < 8; ++i) v[at + i] = 0.0f;
         } else if constexpr (sizeof(T) == 2) {
             const uint4 raw = *reinterpret_cast<const uint4*>(row + first);
             const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(words[i] << 16);
-                v[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u);
+                v[at + 2 * i] = __uint_as_float(words[i] << 16);
+                v[at + 2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u);
             }
         } else {
             const float4 low = *reinterpret_cast<const float4*>(row + first), high = *reinterpret_cast<const float4*>(row + first + 4);
-            v[0] = low.x, v[1] = low.y, v[2] = low.z, v[3] = low.w, v[4] = high.x, v[5] = high.y, v[6] = high.z, v[7] = high.w;
+            v[at + 0] = low.x, v[at + 1] = low.y, v[at + 2] = low.z, v[at + 3] = low.w, v[at + 4] = high.x, v[at + 5] = high.y, v[at + 6] = high.z, v[at + 7] = high.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = first + i < width ? to_float(row[first + i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) v[at + i] = first + i < width ? to_float(row[first + i]) : 0.0f;
     }
 }
 
