@@ -2633,6 +2633,14 @@ def _check_here(what: str, *tensors: "torch.Tensor | None") -> None:
             raise KernelError(f"{what}: a tensor lies on device {tensor.get_device()}, the current device is {device}")
 
 
+def _refuse_gradients(what: str, *tensors: "torch.Tensor | None") -> None:
+    """Refuses tensors that autograd follows: what comes out would lose their gradients without a word."""
+    if torch.is_grad_enabled():
+        for tensor in tensors:
+            if tensor is not None and tensor.requires_grad:
+                raise KernelError(f"{what}: there is no backward pass (detach the tensors, or call it under torch.no_grad())")
+
+
 def microscale(x: torch.Tensor, bits: int = 8) -> Microscaled:
     """Rows ``x`` (bfloat16 or float32, ``[rows, width]``) in microscaled form.  The scale of a block of 32 columns is
     ``2^(floor(log2(max |x|)) - e)`` with the exponent ``e`` of the format's largest element (8 of 448, 2 of 6), at least ``2^-127``; its elements
@@ -2644,6 +2652,7 @@ def microscale(x: torch.Tensor, bits: int = 8) -> Microscaled:
     if x.dim() != 2 or x.shape[1] < 1:
         raise KernelError(f"microscale: x must be [rows, width], got {tuple(x.shape)}")
     code = dtype_code(x.dtype)
+    _refuse_gradients("microscale", x)
     rows, width = x.shape
     out = Microscaled._empty(rows, width, bits, x)
     if rows:
@@ -2667,30 +2676,27 @@ def rmsnorm_microscaled(x: torch.Tensor, weight: torch.Tensor, eps: float, *, de
     rows, width = shape
     if weight.shape != (width,):
         raise KernelError("rmsnorm_microscaled: weight must have one element per column")
-    code = 0
+    x_at, weight_at, delta_at, sum_at, code = x.data_ptr(), weight.data_ptr(), 0, 0, 0
     if delta is not None:
         _check(delta, "delta")
         if delta.shape != shape:
             raise KernelError("rmsnorm_microscaled: delta and x differ in shape")
-        code = dtype_code(delta.dtype)
+        code, delta_at = dtype_code(delta.dtype), delta.data_ptr()
     if sum_out is not None:
         _check(sum_out, "sum_out", torch.float32)
         if sum_out.shape != shape:
             raise KernelError("rmsnorm_microscaled: sum_out and x differ in shape")
-        # between two addresses: the bytes from the lower one on that may not reach the other
-        size, own = 4 * rows * width, sum_out.data_ptr()
-        other, scale = own - x.data_ptr(), own - weight.data_ptr()
-        shares = -size < other < size and other != 0 or -size < scale < 4 * width
-        if delta is not None:
-            other = own - delta.data_ptr()
-            shares = shares or -size < other < delta.itemsize * rows * width
-        if shares and rows:
+        sum_at, size = sum_out.data_ptr(), 4 * rows * width
+        # bytes that two tensors share: the one begins before the other ends, and the other way round
+        shares = -size < sum_at - x_at < size and sum_at != x_at or -size < sum_at - weight_at < 4 * width
+        if shares or delta is not None and -size < sum_at - delta_at < (4 if code == 0 else 2) * rows * width:
             raise KernelError("rmsnorm_microscaled: sum_out may be x, but not overlap it otherwise, nor delta or weight")
     _check_here("rmsnorm_microscaled", x, weight, delta, sum_out)
+    _refuse_gradients("rmsnorm_microscaled", x, weight, delta, sum_out)
     out = Microscaled._empty(rows, width, bits, x)
     if rows:
         codes, scales = out._addresses("rmsnorm_microscaled")
-        _done(_lib().lb_rmsnorm_microscaled(x, delta, sum_out, weight, scale_offset, eps, codes, scales, rows, width, bits, code, _stream()), "rmsnorm_microscaled")
+        _done(_lib().lb_rmsnorm_microscaled(x_at, delta_at, sum_at, weight_at, scale_offset, eps, codes, scales, rows, width, bits, code, _stream()), "rmsnorm_microscaled")
     return out
 
 

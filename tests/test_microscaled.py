@@ -194,3 +194,15 @@ def test_the_plain_implementation():
         codes, scale_bytes = plain.quantise(torch.randn(130, 300), bits)
         back = plain.unpack(*plain.pack(codes, scale_bytes, bits), bits)
         assert torch.equal(back[0], codes) and torch.equal(back[1], scale_bytes)
+
+
+def test_tensors_that_autograd_follows():
+    x, weight = on_cuda(torch.zeros(3, 200)), on_cuda(torch.zeros(200))
+    followed, followed_weight = on_cuda(torch.zeros(3, 200)).requires_grad_(), on_cuda(torch.zeros(200)).requires_grad_()
+    with pytest.raises(ops.KernelError, match="backward"):
+        ops.microscale(followed)
+    for changed in ({"x": followed}, {"weight": followed_weight}, {"delta": followed}):
+        with pytest.raises(ops.KernelError, match="backward"):
+            ops.rmsnorm_microscaled(**{"x": x, "weight": weight, "eps": 1e-5, **changed})
+    with torch.no_grad(), pytest.raises(AssertionError, match="lb_microscale"):
+        ops.microscale(followed)

@@ -247,6 +247,56 @@ def test_a_row_that_is_no_number_stays_in_its_row(tokens):
     assert torch.isnan(hidden[1]).all() and torch.isfinite(hidden[others]).all()
 
 
+@pytest.mark.parametrize("tokens", [3, 200, 1000])
+def test_a_weight_that_is_no_number_stays_in_its_rows(tokens):
+    """Of the product in its column, of a gated product in its channel's block of 32."""
+    generator = torch.Generator().manual_seed(4)
+    w, x = torch.randn(200, 256, generator=generator), torch.randn(tokens, 256, generator=generator)
+    w[70, 200] = float("inf")
+    weight, rows, clean = ops.microscale(w.to(DEVICE), 4), ops.microscale(x.to(DEVICE)), ops.microscale(torch.randn(200, 256, generator=generator).to(DEVICE), 4)
+    out = ops.linear_microscaled(rows, weight).cpu()
+    assert torch.isnan(out[:, 70]).all() and torch.isfinite(out[:, :70]).all() and torch.isfinite(out[:, 71:]).all()
+    for up, gate in ((weight, clean), (clean, weight)):
+        hidden = ops.gated_linear_microscaled(rows, up, gate, "silu").values().cpu()
+        assert torch.isnan(hidden[:, 64:96]).all() and torch.isfinite(hidden[:, :64]).all() and torch.isfinite(hidden[:, 96:]).all()
+
+
+@pytest.mark.parametrize("tokens,rows", [(700, 1700), (4000, 520), (1030, 4608), (2500, 1000)])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_many_tiles(tokens, rows, bits):
+    """More tiles than multiprocessors, wide and narrow ones, the last cut short: whole numbers, so one right result."""
+    x_codes, x_bytes, x = whole_numbers(tokens, 300, bits, tokens)
+    w_codes, w_bytes, w = whole_numbers(rows, 300, 4, rows)
+    want = (x.to(DEVICE) @ w.T.to(DEVICE))
+    given_x, given_w = given(x_codes, x_bytes, 300, bits), given(w_codes, w_bytes, 300, 4)
+    for dtype in (torch.float32, torch.bfloat16):
+        assert torch.equal(ops.linear_microscaled(given_x, given_w, dtype), want.to(dtype))
+    hidden = ops.gated_linear_microscaled(given_x, given_w, given_w, "identity")
+    codes, scale_bytes = plain.quantise((want.float() * want.float()).cpu(), 8)   # both sides are exact in 32 bits, their product is rounded to them once
+    got_codes, got_bytes = made(hidden)
+    assert torch.equal(got_bytes, scale_bytes) and torch.equal(got_codes, codes)
+
+
+def test_rows_past_4_gigabytes():
+    """Elements, codes and outputs whose places need more than 32 bits: the last rows as in a call of their own."""
+    rows, width = 67000, 65536
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device=DEVICE)
+    x[-130:] = torch.randn(130, width, generator=torch.Generator().manual_seed(1)).to(DEVICE, torch.bfloat16)
+    many, few = ops.microscale(x), ops.microscale(x[-130:].clone())
+    assert torch.equal(many.codes[-130:], few.codes)
+    values = many.values()
+    assert torch.equal(values[-130:], few.values()) and not values[:-130].any()
+    del values, x
+    weight = ops.microscale(torch.randn(40, width, generator=torch.Generator().manual_seed(2)).to(DEVICE), 4)
+    out = ops.linear_microscaled(many, weight, torch.float32)
+    want = few.values(torch.float32).double() @ weight.values(torch.float32).double().T
+    sizes = few.values(torch.float32).double().abs() @ weight.values(torch.float32).double().abs().T
+    assert not out[:-130].any()
+    assert bool(((out[-130:].double() - want).abs() <= width * 2.0**-23 * sizes).all())
+
+
 # ------------------------------------------------------------------------------------------------------------------ together
 
 
