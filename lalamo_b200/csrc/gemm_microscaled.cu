@@ -427,31 +427,35 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                     if (issuer) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // the store before last has read this buffer
                     named_barrier(set_barrier, 128);
                     const int token_here = quarter * 4 + (lane >> 3), part = lane & 7;
-                    float h[2][4];
-                    int byte[2];
+                    float up[8], gate[8], h[8];   // four of each of the two blocks
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
                         const float* from = turned + token_here * kMsTurnedPitch + b * 32 + part * 4;
                         const float4 u = *reinterpret_cast<const float4*>(from), g = *reinterpret_cast<const float4*>(from + kMsRows / 2);
-                        h[b][0] = gated_up_side(u.x, p.activation, p.limit) * gated_gate_side(g.x, p.activation, p.limit);
-                        h[b][1] = gated_up_side(u.y, p.activation, p.limit) * gated_gate_side(g.y, p.activation, p.limit);
-                        h[b][2] = gated_up_side(u.z, p.activation, p.limit) * gated_gate_side(g.z, p.activation, p.limit);
-                        h[b][3] = gated_up_side(u.w, p.activation, p.limit) * gated_gate_side(g.w, p.activation, p.limit);
-                        if (row0 + kMsRows / 2 > p.n) {   // past the last row: zeros, whatever the scales there
+                        up[4 * b] = u.x, up[4 * b + 1] = u.y, up[4 * b + 2] = u.z, up[4 * b + 3] = u.w;
+                        gate[4 * b] = g.x, gate[4 * b + 1] = g.y, gate[4 * b + 2] = g.z, gate[4 * b + 3] = g.w;
+                    }
+                    gated_values(up, gate, p.activation, p.limit, h);
+                    if (row0 + kMsRows / 2 > p.n) {   // past the last row: zeros, whatever the scales there
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (row0 + b * 32 + part * 4 + i >= p.n) h[b][i] = 0.0f;
-                        }
+                        for (int i = 0; i < 8; ++i)
+                            if (row0 + (i >> 2) * 32 + part * 4 + (i & 3) >= p.n) h[i] = 0.0f;
+                    }
+                    float largest[2];
+                    int byte[2];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) largest[b] = larger_size(larger_size(h[4 * b], h[4 * b + 1]), larger_size(h[4 * b + 2], h[4 * b + 3]));
+#pragma unroll
+                    for (int offset = 1; offset < 8; offset <<= 1) {
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) largest[b] = larger_size(largest[b], __shfl_xor_sync(0xffffffffu, largest[b], offset));
                     }
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
-                        float largest = larger_size(larger_size(h[b][0], h[b][1]), larger_size(h[b][2], h[b][3]));
-#pragma unroll
-                        for (int offset = 1; offset < 8; offset <<= 1) largest = larger_size(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
-                        byte[b] = scale_byte<8>(__float_as_uint(largest) & 0x7fffffffu);
+                        byte[b] = scale_byte<8>(__float_as_uint(largest[b]) & 0x7fffffffu);
                         const float inverse = scale_inverse(byte[b]);
                         *reinterpret_cast<uint32_t*>(out_buffer + token_here * 64 + b * 32 + part * 4) =
-                            pack_e4m3(h[b][0] * inverse, h[b][1] * inverse, h[b][2] * inverse, h[b][3] * inverse);
+                            pack_e4m3(h[4 * b] * inverse, h[4 * b + 1] * inverse, h[4 * b + 2] * inverse, h[4 * b + 3] * inverse);
                     }
                     const int token = first_token + token_here, block = row0 / 32;   // an even one
                     if (part == 0 && token < p.tokens)
@@ -758,12 +762,12 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
             float4 sums[2];
             add_up(at, at + kMsRows / 2, sums);
             const float up[4] = {sums[0].x, sums[0].y, sums[0].z, sums[0].w}, gate[4] = {sums[1].x, sums[1].y, sums[1].z, sums[1].w};
-            float h[4], largest = 0.0f;
+            float h[4];
+            gated_values(up, gate, p.activation, p.limit, h);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                h[e] = row0 + channel + e < p.n ? gated_up_side(up[e], p.activation, p.limit) * gated_gate_side(gate[e], p.activation, p.limit) : 0.0f;
-                largest = larger_size(largest, h[e]);
-            }
+            for (int e = 0; e < 4; ++e)
+                if (row0 + channel + e >= p.n) h[e] = 0.0f;
+            float largest = larger_size(larger_size(h[0], h[1]), larger_size(h[2], h[3]));
 #pragma unroll
             for (int offset = 1; offset < 8; offset <<= 1) largest = larger_size(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
             const int byte = scale_byte<8>(__float_as_uint(largest) & 0x7fffffffu);

@@ -132,18 +132,27 @@ __device__ __forceinline__ void store_codes(unsigned char* to, const uint32_t (&
     else *reinterpret_cast<uint32_t*>(to) = codes[0];
 }
 
-// What the gate side of a gated product multiplies with, and the up side.
-__device__ __forceinline__ float gated_gate_side(float g, int activation, float limit) {
-    if (activation == kSigmoidLimit) {
-        const float c = fminf(g, limit);
-        return __fdividef(c, 1.0f + __expf(-kSigmoidLimitSlope * c));
+// values = up * act(gate), in 32 bits, of the activations 0 silu, 1 gelu (erf), 2 identity; 3: min(gate, limit) * sigmoid(1.702 min(gate, limit)) * (clamp(up, -limit,
+// limit) + 1).  The choice lies outside the loops, so that the values' exponentials and divisions overlap (inside, a gated product of 777 tokens, 6912 x 1536, took
+// 22.3 us).
+template <int COUNT>
+__device__ __forceinline__ void gated_values(const float (&up)[COUNT], const float (&gate)[COUNT], int activation, float limit, float (&values)[COUNT]) {
+    if (activation == 0) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) values[i] = up[i] * __fdividef(gate[i], 1.0f + __expf(-gate[i]));
+    } else if (activation == 1) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) values[i] = up[i] * (0.5f * gate[i] * (1.0f + erff(gate[i] * 0.70710678118654752440f)));
+    } else if (activation == kSigmoidLimit) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const float g = fminf(gate[i], limit);
+            values[i] = (fminf(fmaxf(up[i], -limit), limit) + 1.0f) * __fdividef(g, 1.0f + __expf(-kSigmoidLimitSlope * g));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) values[i] = up[i] * gate[i];
     }
-    if (activation == 0) return __fdividef(g, 1.0f + __expf(-g));
-    if (activation == 1) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752440f));
-    return g;
-}
-__device__ __forceinline__ float gated_up_side(float u, int activation, float limit) {
-    return activation == kSigmoidLimit ? fminf(fmaxf(u, -limit), limit) + 1.0f : u;
 }
 
 // Eight columns from `first` of a row of `width`, as float32, into v[at] on; past the width zeros.  VECTOR: the row starts on 16 bytes and the width is a multiple of 8.

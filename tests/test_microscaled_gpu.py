@@ -277,6 +277,17 @@ def test_many_tiles(tokens, rows, bits):
     assert torch.equal(got_bytes, scale_bytes) and torch.equal(got_codes, codes)
 
 
+@pytest.mark.parametrize("tokens,rows", [(393, 4931), (643, 4873)])
+def test_tiles_of_two_multiprocessors(tokens, rows):
+    """Rows of 8 bits and a K long enough for pairs of CTAs, an odd number of 128 rows of the weight, and a last tile of 73 tokens and of 3."""
+    x_codes, x_bytes, x = whole_numbers(tokens, 8192, 8, tokens)
+    w_codes, w_bytes, w = whole_numbers(rows, 8192, 4, rows)
+    want = x.to(DEVICE) @ w.T.to(DEVICE)
+    given_x, given_w = given(x_codes, x_bytes, 8192, 8), given(w_codes, w_bytes, 8192, 4)
+    for dtype in (torch.float32, torch.bfloat16):
+        assert torch.equal(ops.linear_microscaled(given_x, given_w, dtype), want.to(dtype))
+
+
 def test_rows_past_4_gigabytes():
     """Elements, codes and outputs whose places need more than 32 bits: the last rows as in a call of their own."""
     rows, width = 67000, 65536
