@@ -539,13 +539,9 @@ struct MsSplit {
     static constexpr int kSlack = 1024 + 256;             // alignment and barriers
     static constexpr int kRoom = (kMsSplitShared - kSlack) / MsShape<BITS, BN>::kStageBytes;
     static constexpr int kMostStages = kRoom < kMsSplitStages ? kRoom : kMsSplitStages;
-    // A CTA waits for tensor memory without a limit, and one of a cluster keeps it until the others are done: clusters that wait for one another's would never
-    // end.  So a CTA takes at least that part of a multiprocessor's shared memory that it takes of its 512 columns, and what fits the one fits the other.
-    static constexpr int kLeast = kColumns * (kMsSharedLimit / 512) - 2048 < kMsSplitShared ? kColumns * (kMsSharedLimit / 512) - 2048 : kMsSplitShared;
-    static_assert(kColumns < 256 || kLeast + 2048 >= kMsSharedLimit / 2, "two CTAs of 256 columns leave no room for a third");
     static int bytes(int stages) {
-        const int ring = stages * MsShape<BITS, BN>::kStageBytes, needed = (ring > kPartBytes ? ring : kPartBytes) + kSlack;
-        return needed > kLeast ? needed : kLeast;
+        const int ring = stages * MsShape<BITS, BN>::kStageBytes;
+        return (ring > kPartBytes ? ring : kPartBytes) + kSlack;
     }
 };
 
@@ -689,11 +685,11 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
             atomicExch(&failed, 1);
         }
     }
+    // Tensor memory goes back before the CTAs wait for one another: one that waits to get some, without a limit, never waits for a CTA that waits for it.
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncwarp();
-    // all parts are there, or some CTA has failed and says so below
-    if (splits > 1) cluster_sync();
-    else __syncthreads();
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Split::kColumns) : "memory");
+    if (splits > 1) cluster_sync();   // all parts are there, or some CTA has failed and says so below
     const int tokens_here = min(BN, p.tokens - token0);
     const uint32_t part = smem_address(ring);
     // Four rows (of a token) at each of two places, part after part; all parts are read before the first is added.
@@ -789,7 +785,6 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
     // Nobody leaves while another still reads its part.  Nothing is to be ordered by it: what has been read is in registers (add_up sees to it), the output is of no
     // concern to the others, and an arrival that waited for its writes would take some 800 cycles more.
     if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Split::kColumns) : "memory");
 }
 
 // Codes as boxes of [box_rows, 128 bytes of shared memory] with 128-byte swizzle; `spread`: 4-bit elements to 16 in 16 bytes (boxes of 128 elements),
