@@ -38,8 +38,9 @@ __device__ __forceinline__ void bulk_load(void* destination, const void* source,
                  : "memory");
 }
 
-// True in one lane of the warp.  The copying and the issuing warp walk their loops as a whole, and one lane, elected each time, issues: inside a branch on the
+// True in one lane of the warp.  The copying and the issuing warp walk their loops as a whole, and an elected lane issues: inside a branch on the
 // lane's number the same instructions took 55 cycles each, which bounded a stage of the ring at 500.
+// (The same lane is elected every time, so that products keep their order and a commit counts them.)
 __device__ __forceinline__ bool elect_lane() {
     uint32_t elected;
     asm volatile(
@@ -131,20 +132,22 @@ struct MsShape {
     static constexpr uint32_t kWCounted = BITS == 8 ? kWBytes / 2 : kWBytes;
 };
 
-// One lane's work: a landed stage's scales to a set of columns of tensor memory,
+// A landed stage's scales to a set of columns of tensor memory.  The whole warp comes here, and a lane is elected for every instruction (gated 8192 x 2048, 8 tokens:
+// 6.5 us, and 7.1 with one lane for all of a stage); for a pair one lane comes, elected for all of them (4,096 tokens, 2048 x 8192: 61 us, and 96 with one each).
 template <typename Shape, bool PAIR>
 __device__ __forceinline__ void copy_stage_scales(const unsigned char* stage, uint32_t columns, int chunks) {
     const unsigned char* scales = stage + Shape::kWBytes + Shape::kXBytes;
 #pragma unroll
     for (int c = 0; c < Shape::kChunks; ++c) {
         if (c >= chunks) break;
-        copy_scales<PAIR>(columns + 4 * c, scales + c * kScaleTileBytes);
+        if (PAIR || elect_lane()) copy_scales<PAIR>(columns + 4 * c, scales + c * kScaleTileBytes);
 #pragma unroll
         for (int t = 0; t < Shape::kScaleTiles; ++t)
-            copy_scales<PAIR>(columns + 4 * (Shape::kChunks + c * Shape::kScaleTiles + t), scales + Shape::kWScaleBytes + (t * Shape::kChunks + c) * kScaleTileBytes);
+            if (PAIR || elect_lane())
+                copy_scales<PAIR>(columns + 4 * (Shape::kChunks + c * Shape::kScaleTiles + t), scales + Shape::kWScaleBytes + (t * Shape::kChunks + c) * kScaleTileBytes);
     }
 }
-// and its four products under them, and the stage's return to the producer(s).
+// Its four products under them, and the stage's return to the producer(s), likewise.
 template <int BITS, typename Shape, bool PAIR>
 __device__ __forceinline__ void issue_stage(uint32_t tmem_d, const unsigned char* stage, uint32_t columns, uint32_t token_column, uint32_t idesc, int chunks, bool accumulate,
                                             uint64_t* empty) {
@@ -153,11 +156,14 @@ __device__ __forceinline__ void issue_stage(uint32_t tmem_d, const unsigned char
     for (int k = 0; k < 4; ++k) {
         const int c = product_chunk<BITS>(k);
         if (c >= chunks) break;
-        mma_microscaled<BITS, PAIR>(tmem_d, desc_w + 2 * k, desc_x + 2 * k, idesc | product_scales<BITS>(k), columns + 4 * c,
-                                    columns + 4 * (Shape::kChunks + c * Shape::kScaleTiles) + token_column, accumulate || k > 0);
+        if (PAIR || elect_lane())
+            mma_microscaled<BITS, PAIR>(tmem_d, desc_w + 2 * k, desc_x + 2 * k, idesc | product_scales<BITS>(k), columns + 4 * c,
+                                        columns + 4 * (Shape::kChunks + c * Shape::kScaleTiles) + token_column, accumulate || k > 0);
     }
-    if constexpr (PAIR) mma_commit_pair(empty);
-    else mma_commit(empty);
+    if (PAIR || elect_lane()) {
+        if constexpr (PAIR) mma_commit_pair(empty);
+        else mma_commit(empty);
+    }
 }
 
 constexpr int kMsWide = 192, kMsNarrow = 128;   // tokens of the walking kernel's tiles, which begin at multiples of 64
@@ -302,14 +308,8 @@ gemm_microscaled_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                     ok = barrier_wait_warp(&full[s], round & 1);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    // In one branch or in two: with rows of 8 bits two are sooner done (2048 tokens, 2048 x 8192: 35.9 us and 38.0), with 4 bits one (20.6 and 22.6).
-                    if constexpr (BITS == 8) {
-                        if (elect_lane()) copy_stage_scales<Shape, false>(at, tmem_scales, chunks_of(stage));
-                        if (elect_lane()) issue_stage<BITS, Shape, false>(tmem_d, at, tmem_scales, token_column, idesc, chunks_of(stage), stage > 0, &empty[s]);
-                    } else if (elect_lane()) {
-                        copy_stage_scales<Shape, false>(at, tmem_scales, chunks_of(stage));
-                        issue_stage<BITS, Shape, false>(tmem_d, at, tmem_scales, token_column, idesc, chunks_of(stage), stage > 0, &empty[s]);
-                    }
+                    copy_stage_scales<Shape, false>(at, tmem_scales, chunks_of(stage));
+                    issue_stage<BITS, Shape, false>(tmem_d, at, tmem_scales, token_column, idesc, chunks_of(stage), stage > 0, &empty[s]);
                     if (++s == STAGES) s = 0, ++round;
                 } else {
                     // A pair's scales of the stage after go out before this stage's products if that stage is there (4096 tokens x 2048 x 8192: 60.8 us, and 65.4 with
@@ -624,11 +624,9 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
             ok = barrier_wait_warp(&full[s], round & 1);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (elect_lane()) {
-                const unsigned char* at = ring + s * Shape::kStageBytes;
-                copy_stage_scales<Shape, false>(at, tmem_base + BN, chunks_of(first_stage + i));
-                issue_stage<BITS, Shape, false>(tmem_base, at, tmem_base + BN, static_cast<uint32_t>((token0 & 127) >> 5), idesc, chunks_of(first_stage + i), i > 0, &empty[s]);
-            }
+            const unsigned char* at = ring + s * Shape::kStageBytes;
+            copy_stage_scales<Shape, false>(at, tmem_base + BN, chunks_of(first_stage + i));
+            issue_stage<BITS, Shape, false>(tmem_base, at, tmem_base + BN, static_cast<uint32_t>((token0 & 127) >> 5), idesc, chunks_of(first_stage + i), i > 0, &empty[s]);
             if (++s == ring_stages) s = 0, ++round;
         }
         if (!ok) atomicExch(&failed, 1);
