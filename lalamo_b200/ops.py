@@ -2635,10 +2635,9 @@ def _check_here(what: str, *tensors: "torch.Tensor | None") -> None:
 
 def _refuse_gradients(what: str, *tensors: "torch.Tensor | None") -> None:
     """Refuses tensors that autograd follows: what comes out would lose their gradients without a word."""
-    if torch.is_grad_enabled():
-        for tensor in tensors:
-            if tensor is not None and tensor.requires_grad:
-                raise KernelError(f"{what}: there is no backward pass (detach the tensors, or call it under torch.no_grad())")
+    for tensor in tensors:
+        if tensor is not None and tensor.requires_grad:
+            raise KernelError(f"{what}: there is no backward pass (detach the tensors, or call it under torch.no_grad())")
 
 
 def microscale(x: torch.Tensor, bits: int = 8) -> Microscaled:
@@ -2652,7 +2651,8 @@ def microscale(x: torch.Tensor, bits: int = 8) -> Microscaled:
     if x.dim() != 2 or x.shape[1] < 1:
         raise KernelError(f"microscale: x must be [rows, width], got {tuple(x.shape)}")
     code = dtype_code(x.dtype)
-    _refuse_gradients("microscale", x)
+    if x.requires_grad and torch.is_grad_enabled():
+        _refuse_gradients("microscale", x)
     rows, width = x.shape
     out = Microscaled._empty(rows, width, bits, x)
     if rows:
@@ -2691,8 +2691,12 @@ def rmsnorm_microscaled(x: torch.Tensor, weight: torch.Tensor, eps: float, *, de
         shares = -size < sum_at - x_at < size and sum_at != x_at or -size < sum_at - weight_at < 4 * width
         if shares or delta is not None and -size < sum_at - delta_at < (4 if code == 0 else 2) * rows * width:
             raise KernelError("rmsnorm_microscaled: sum_out may be x, but not overlap it otherwise, nor delta or weight")
-    _check_here("rmsnorm_microscaled", x, weight, delta, sum_out)
-    _refuse_gradients("rmsnorm_microscaled", x, weight, delta, sum_out)
+    device = _current_device()
+    if (x.get_device() != device or weight.get_device() != device or delta is not None and delta.get_device() != device
+            or sum_out is not None and sum_out.get_device() != device):
+        _check_here("rmsnorm_microscaled", x, weight, delta, sum_out)
+    if torch.is_grad_enabled():
+        _refuse_gradients("rmsnorm_microscaled", x, weight, delta, sum_out)
     out = Microscaled._empty(rows, width, bits, x)
     if rows:
         codes, scales = out._addresses("rmsnorm_microscaled")
