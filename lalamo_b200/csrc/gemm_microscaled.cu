@@ -17,6 +17,7 @@
 namespace lb {
 
 constexpr int kMsRows = 128;   // lanes of an accumulator
+constexpr int kMsMostRows = 0x7fffff00;   // of either operand: places are counted in whole tiles
 
 struct MsParams {
     const unsigned char *w_scales, *gate_scales, *x_scales;
@@ -96,9 +97,9 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, const void* tile) {
         : "memory")
 template <int BITS, bool PAIR>
 __device__ __forceinline__ void mma_microscaled(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t scales_a, uint32_t scales_b, bool accumulate) {
-    if constexpr (BITS == 8 && PAIR) LB_MMA_MICROSCALED("2", "mxf8f6f4", "1X");
+    static_assert(!PAIR || BITS == 8, "what pairs take");
+    if constexpr (PAIR) LB_MMA_MICROSCALED("2", "mxf8f6f4", "1X");
     else if constexpr (BITS == 8) LB_MMA_MICROSCALED("1", "mxf8f6f4", "1X");
-    else if constexpr (PAIR) LB_MMA_MICROSCALED("2", "mxf4", "2X");
     else LB_MMA_MICROSCALED("1", "mxf4", "2X");
 }
 #undef LB_MMA_MICROSCALED
@@ -913,23 +914,26 @@ int launch_microscaled_split(const void* x, const void* w, const void* gate, MsP
     return static_cast<int>(cudaLaunchKernelEx(&config, kernel, map_w, map_gate, map_x, p, splits, per_split, ring));
 }
 
-// How the tokens are cut into tiles: of all numbers of tiles, the first as many of them wide as it takes, the one whose first walker, which has the most and the widest
-// tiles, is done first.  What a stage of K costs (hundredths of a microsecond, measured at 4,096 tokens, 2048 x 8192, under sustained load): 29 with 128 tokens and 36
-// with 192; of a pair 27 and 32; with rows of 4 bits 30 and 36.
+// How the tokens are cut into tiles: of all numbers of tiles, the first as many of them wide as it takes, or one more, which leaves fewer tokens to the last, the cut whose first
+// walker, which has the most and the widest tiles, is done first.  What a stage of K costs (hundredths of a microsecond, measured at 4,096 tokens, 2048 x 8192, under
+// sustained load): 29 with 128 tokens and 36 with 192; of a pair 27 and 32; with rows of 4 bits 30 and 36.
 struct TokenTiles {
     int count, wide;
     long long cost;   // of the walk
 };
 inline TokenTiles cut_tokens(int tokens, long long row_tiles, int walkers, long long stages, int narrow_cost, int wide_cost) {
+    constexpr int kStep = kMsWide - kMsNarrow;
     TokenTiles best = {0, 0, -1};
+    const auto rounds = [&](int tiles) { return (row_tiles * tiles + walkers - 1) / walkers; };   // of the first walker that begin before so many of the tokens' tiles end
     for (int count = (tokens + kMsWide - 1) / kMsWide; count <= (tokens + kMsNarrow - 1) / kMsNarrow; ++count) {
-        const int more = tokens - count * kMsNarrow, step = kMsWide - kMsNarrow, wide = more > 0 ? (more + step - 1) / step : 0;
-        const int last = tokens - ((count - 1) * kMsNarrow + min(wide, count - 1) * step);   // tokens of the last tile
-        // rounds of the first walker: all, those that begin before the last tile, and of these those with a wide tile
-        const auto rounds = [&](int tiles) { return (row_tiles * tiles + walkers - 1) / walkers; };
-        const long long before = rounds(count - 1), wides = min(rounds(min(wide, count - 1)), before);
-        const long long cost = wides * wide_cost + (before - wides) * narrow_cost + (rounds(count) - before) * (narrow_cost + (last - kMsNarrow) * (wide_cost - narrow_cost) / step);
-        if (best.cost < 0 || cost * stages < best.cost) best = {count, wide, cost * stages};
+        const int more = tokens - count * kMsNarrow, least = more > 0 ? (more + kStep - 1) / kStep : 0;
+        for (int wide = least; wide <= min(least + 1, count); ++wide) {
+            const int last = tokens - ((count - 1) * kMsNarrow + min(wide, count - 1) * kStep);   // tokens of the last tile
+            if (last < 1) break;
+            const long long before = rounds(count - 1), wides = min(rounds(min(wide, count - 1)), before);
+            const long long cost = wides * wide_cost + (before - wides) * narrow_cost + (rounds(count) - before) * (narrow_cost + (last - kMsNarrow) * (wide_cost - narrow_cost) / kStep);
+            if (best.cost < 0 || cost * stages < best.cost) best = {count, wide, cost * stages};
+        }
     }
     return best;
 }
@@ -961,7 +965,7 @@ extern "C" {
 // Returns 0, a CUDA error, -2 for sizes or addresses that the kernel does not take, -5 if no tensor map could be made.
 int lb_gemm_microscaled(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int tokens, int n, int chunks, int bits, int out_is_float,
                         int* status, cudaStream_t stream) {
-    if (tokens < 1 || n < 1 || chunks < 1 || chunks > (1 << 22) || (bits != 4 && bits != 8)) return -2;
+    if (tokens < 1 || tokens > lb::kMsMostRows || n < 1 || n > lb::kMsMostRows || chunks < 1 || chunks > (1 << 22) || (bits != 4 && bits != 8)) return -2;
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(w_scales)) & 15 || reinterpret_cast<uintptr_t>(w) & 31) return -2;
     lb::MsParams p = {};
     p.w_scales = static_cast<const unsigned char*>(w_scales);
@@ -978,7 +982,7 @@ int lb_gemm_microscaled(const void* x, const void* x_scales, const void* w, cons
 // codes and scales of (x up^T) * act(x gate^T) in 8 bits: [tokens, n made up to whole 128s].
 int lb_gated_microscaled(const void* x, const void* x_scales, const void* up, const void* up_scales, const void* gate, const void* gate_scales, void* out, void* out_scales,
                          int tokens, int n, int chunks, int bits, int activation, float limit, int* status, cudaStream_t stream) {
-    if (tokens < 1 || n < 1 || chunks < 1 || chunks > (1 << 22) || (bits != 4 && bits != 8) || activation < 0 || activation > 3) return -2;
+    if (tokens < 1 || tokens > lb::kMsMostRows || n < 1 || n > lb::kMsMostRows || chunks < 1 || chunks > (1 << 22) || (bits != 4 && bits != 8) || activation < 0 || activation > 3) return -2;
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(up_scales) | reinterpret_cast<uintptr_t>(gate_scales) |
          reinterpret_cast<uintptr_t>(out)) & 15 || (reinterpret_cast<uintptr_t>(up) | reinterpret_cast<uintptr_t>(gate)) & 31)
         return -2;
