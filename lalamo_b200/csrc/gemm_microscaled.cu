@@ -887,8 +887,10 @@ int launch_microscaled_split(const void* x, const void* w, const void* gate, MsP
     const int row_tiles = GATED ? p.out_chunks * 2 : (p.n + kMsRows - 1) / kMsRows, token_tiles = (p.tokens + BN - 1) / BN, sms = multiprocessor_count();
     const int stages = (p.chunks + MsShape<BITS, BN>::kChunks - 1) / MsShape<BITS, BN>::kChunks;
     // Two CTAs fit a multiprocessor: clusters of eight that have one each do not all find room at once (2048 x 8192 and a token: 9.1 us, and 5.0 with room for two),
-    // and a deeper ring gains nothing.  With 128 tokens the sums to be read from eight CTAs cost more than their stages gain (four: 9.1 us, eight: 12.1).
-    int wanted = max(1, min(min(sms / (row_tiles * token_tiles), BN > 64 ? kMsLargestSplit / 2 : kMsLargestSplit), stages));
+    // and a deeper ring gains nothing.  A stage takes 0.18 us, a meeting of up to four CTAs 0.6 us and of eight 1.2, more with more tokens: beyond four where each still has
+    // three stages (8 tokens, 2048 x 2048: 3.4 us by four, 3.8 by eight; 1024 x 4608 4.6 and 3.9), and of more than 32 tokens six at most (128 tokens, 2048 x 8192: 10.5 us by
+    // four, 9.6 by six, 11.3 by eight).
+    int wanted = max(1, min(min(sms / (row_tiles * token_tiles), stages), min(max(4, stages / 3), BN > 32 ? 6 : kMsLargestSplit)));
     // Gated tiles that nearly fill the multiprocessors are cut in two all the same, two CTAs to each (8192 x 2048, 64 tokens: 11.3 and 9.4 us; other products lose
     // by it: 6.4 and 7.3).
     if (GATED && wanted == 1 && stages > 1 && row_tiles * token_tiles <= sms && (BITS == 8 || BN > 16)) wanted = 2;
