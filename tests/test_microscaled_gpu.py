@@ -247,6 +247,24 @@ def test_a_row_that_is_no_number_stays_in_its_row(tokens):
     assert torch.isnan(hidden[1]).all() and torch.isfinite(hidden[others]).all()
 
 
+@pytest.mark.parametrize("tokens", [3, 200])
+@pytest.mark.parametrize("activation", ["silu", "gelu", "sigmoid_limit", "identity"])
+def test_no_activation_makes_a_number_of_what_is_none(activation, tokens):
+    """Limits keep numbers within bounds; a NaN in `up` or in `gate` passes them."""
+    generator = torch.Generator().manual_seed(5)
+    x, w = torch.randn(tokens, 256, generator=generator), torch.randn(130, 256, generator=generator)
+    x[1, 3] = float("nan")
+    clean = ops.microscale(w.to(DEVICE), 4)
+    hidden = ops.gated_linear_microscaled(ops.microscale(x.to(DEVICE)), clean, clean, activation, limit=3.0).values().cpu()
+    others = torch.arange(tokens) != 1
+    assert torch.isnan(hidden[1]).all() and torch.isfinite(hidden[others]).all()
+    w[70, 200] = float("nan")
+    weight, rows = ops.microscale(w.to(DEVICE), 4), ops.microscale(torch.randn(tokens, 256, generator=generator).to(DEVICE))
+    for up, gate in ((weight, clean), (clean, weight)):
+        hidden = ops.gated_linear_microscaled(rows, up, gate, activation, limit=3.0).values().cpu()
+        assert torch.isnan(hidden[:, 64:96]).all() and torch.isfinite(hidden[:, :64]).all() and torch.isfinite(hidden[:, 96:]).all()
+
+
 @pytest.mark.parametrize("tokens", [3, 200, 1000])
 def test_a_weight_that_is_no_number_stays_in_its_rows(tokens):
     """Of the product in its column, of a gated product in its channel's block of 32."""
