@@ -687,8 +687,14 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
     // Tensor memory goes back before the CTAs wait for one another: one that waits to get some, without a limit, never waits for a CTA that waits for it.
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (failed) {
+        // Let whatever copies and products are still in flight land before their memories go away.
+        if (threadIdx.x == 0) report_error(p.status, kWaitTimeout);
+        for (int spin = 0; spin < 2000; ++spin) __nanosleep(1000);
+        __syncthreads();
+    }
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Split::kColumns) : "memory");
-    if (splits > 1) cluster_sync();   // all parts are there, or some CTA has failed and says so below
+    if (splits > 1) cluster_sync();   // all parts are there, or some CTA has failed and said so
     const int tokens_here = min(BN, p.tokens - token0);
     const uint32_t part = smem_address(ring);
     // Four rows (of a token) at each of two places, part after part; all parts are read before the first is added.
@@ -775,14 +781,9 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
             }
         }
     }
-    __syncthreads();
-    if (failed) {
-        if (threadIdx.x == 0) report_error(p.status, kWaitTimeout);
-        for (int spin = 0; spin < 2000; ++spin) __nanosleep(1000);
-        __syncthreads();
-    }
     // Nobody leaves while another still reads its part.  Nothing is to be ordered by it: what has been read is in registers (add_up sees to it), the output is of no
     // concern to the others, and an arrival that waited for its writes would take some 800 cycles more.
+    __syncwarp();
     if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
