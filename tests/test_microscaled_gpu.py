@@ -248,6 +248,24 @@ def test_a_row_that_is_no_number_stays_in_its_row(tokens):
 
 
 @pytest.mark.parametrize("tokens", [3, 200])
+@pytest.mark.parametrize("activation", ["silu", "gelu", "sigmoid_limit"])
+def test_activations_of_far_negative_gates(activation, tokens):
+    """A block that has small values only has them as exactly as others.  Its gates g are one whole number down to -6, exact as the values of up are; the exponential of at most
+    1.702 |g| is off by less than 2 + 1.2 * 1.702 |g| last places, erfc by 2 g^2 times the 2^-23 of its argument and 5 more, all of them below (g^2 + 12) 2^-23."""
+    width = 128
+    x = torch.zeros(tokens, width)
+    x[:, 0] = 1.0
+    up, gate = torch.zeros(96, width), torch.zeros(96, width)
+    up[:, 0] = torch.tensor([1.0, 1.5, 2.0])[torch.arange(96) % 3]
+    gate[:, 0] = -torch.tensor([6.0, 4.0, 3.0])[torch.arange(96) // 32]
+    out = ops.gated_linear_microscaled(ops.microscale(x.to(DEVICE)), ops.microscale(up.to(DEVICE), 4), ops.microscale(gate.to(DEVICE), 4), activation, limit=7.0)
+    g = gate[:, 0].double().expand(tokens, -1)
+    h = plain.activate(g, up[:, 0].double().expand(tokens, -1), activation, 7.0)
+    error = h.abs() * (g * g + 12) * 2.0**-23
+    assert between(out.values(torch.float32).cpu().double(), plain.through(h - error, 8), plain.through(h + error, 8))
+
+
+@pytest.mark.parametrize("tokens", [3, 200])
 @pytest.mark.parametrize("activation", ["silu", "gelu", "sigmoid_limit", "identity"])
 def test_no_activation_makes_a_number_of_what_is_none(activation, tokens):
     """Limits keep numbers within bounds; a NaN in `up` or in `gate` passes them."""
