@@ -82,7 +82,6 @@ template <typename T, int BITS, bool VECTOR>
 __global__ void __launch_bounds__(kMicroscaleThreads)
 microscaled_values_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales, T* __restrict__ out, int width, unsigned total, Divisor chunks) {
     wait_for_previous_kernel();
-    allow_next_kernel();
     constexpr int kRounds = kValuesRounds<T>;
     const int column = (threadIdx.x & 15) * 8;
     Piece piece[kRounds];
@@ -108,6 +107,11 @@ microscaled_values_kernel(const unsigned char* __restrict__ codes, const unsigne
         store_eight<VECTOR>(out + static_cast<size_t>(piece[u].row) * width, piece[u].chunk * 128 + column, width, v);
     }
 }
+
+// Nothing, launched the ordinary way behind the values: they may be a weight, and a bfloat16 product asks for its first tiles of W before it waits for the kernel in front of it.
+// It starts when this has ended, and this when the values are written; so does every product after it.  (A kernel that merely does not let its successor start early ends
+// before its writes are seen to.)  Costs 1 us of the device's time.
+__global__ void values_are_written_kernel() {}
 
 // s = x + delta; sum_out = s; y = s * rsqrt(mean(s^2) + eps) * (weight + offset), microscaled from 32 bits.  A block per row, GROUPS pieces of eight
 // columns a thread, which stay in registers between the sum of squares and the norm.  sum_out may be x: an element is read and written by one thread.
@@ -172,8 +176,11 @@ template <typename T, int BITS>
 cudaError_t launch_values(const unsigned char* codes, const unsigned char* scales, T* out, int rows, int width, cudaStream_t stream) {
     const int chunks = (width + 127) / 128;
     auto kernel = rows_are_aligned(out, width) ? microscaled_values_kernel<T, BITS, true> : microscaled_values_kernel<T, BITS, false>;
-    return launch_overlapped(kernel, microscale_grid<16, kValuesRounds<T>>(static_cast<unsigned>(rows) * chunks), dim3(kMicroscaleThreads), 0, stream, codes, scales, out, width,
-                             static_cast<unsigned>(rows) * chunks, divisor_of(chunks));
+    const cudaError_t error = launch_overlapped(kernel, microscale_grid<16, kValuesRounds<T>>(static_cast<unsigned>(rows) * chunks), dim3(kMicroscaleThreads), 0, stream, codes, scales, out,
+                                                width, static_cast<unsigned>(rows) * chunks, divisor_of(chunks));
+    if (error != cudaSuccess) return error;
+    values_are_written_kernel<<<1, 32, 0, stream>>>();
+    return cudaGetLastError();
 }
 
 template <typename TD, int BITS, int GROUPS>

@@ -2381,7 +2381,8 @@ def _product(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
 def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: torch.dtype | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T`` with 32-bit accumulation; ``out_dtype`` float32 gives 32-bit results from
     bfloat16 operands (the LM head's logits).  Steps of up to 16 tokens go to the weight-streaming
-    kernel, everything else to the library."""
+    kernel, everything else to the library.  The kernels may ask for ``weight`` before the one in front of them has ended: what
+    an operator of this module has just written is no weight before a synchronisation, but :meth:`Microscaled.values` are one at once."""
     _check(x, "x")
     _check(weight, "weight", x.dtype)
     rows, width = weight.shape
@@ -2612,12 +2613,12 @@ class Microscaled:
         return self._codes.data_ptr(), self._scales.data_ptr()
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The numbers, ``[rows, width]``: exact in float32, and in bfloat16 down to its subnormals."""
+        """The numbers, ``[rows, width]``: exact in float32, and in bfloat16 down to its subnormals.  They may be a product's weight at once."""
         codes, scales = self._addresses("microscaled_values")
         code = dtype_code(dtype)
         out = (self._store if self._store is not None else self._codes).new_empty((self.rows, self.width), dtype=dtype)
         if self.rows:
-            _done(_lib().lb_microscaled_values(codes, scales, out, self.rows, self.width, self.bits, code, _stream()), "microscaled_values")
+            _done(_lib().lb_microscaled_values(codes, scales, out, self.rows, self.width, self.bits, code, _stream()), "microscaled_values", 2)
         return out
 
 
