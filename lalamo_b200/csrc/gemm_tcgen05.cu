@@ -90,11 +90,6 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(barriers + 2 * STAGES + 1);
     __shared__ int failed;
 
-    // With more than 16 tokens the successor may start early (measured: 1.6 % of a 64-token decode step, 2.7 %
-    // of a 64-token prompt).  With fewer it is a weight-streaming product that pulls its weights towards L2
-    // while this kernel's tiles of W stream in, which cost more than its early start gained (1.05 against
-    // 0.97 ms a step).
-    if (p.early_successor) allow_next_kernel();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // Gated: 64 "up" rows and the 64 "gate" rows that belong to them share the CTA.
     const bool gated = p.epilogue == kTcGated;
@@ -120,6 +115,13 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
+
+    // With more than 16 tokens the successor may start early (measured: 1.6 % of a 64-token decode step, 2.7 %
+    // of a 64-token prompt).  With fewer it is a weight-streaming product that pulls its weights towards L2
+    // while this kernel's tiles of W stream in, which cost more than its early start gained (1.05 against
+    // 0.97 ms a step).
+    // Not before this CTA has its tensor memory: the successor's CTAs may hold some while they wait for this kernel.
+    if (p.early_successor) allow_next_kernel();
 
     if (warp == 0 && lane == 0) {
         // Producer.  The weights do not depend on the kernel before this one: the first round of
@@ -343,7 +345,7 @@ gemm_tcgen05_persistent_kernel(const __grid_constant__ CUtensorMap map_w, const 
     const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
     const int walker = PAIR ? static_cast<int>(blockIdx.x) >> 1 : static_cast<int>(blockIdx.x);
     const int walkers = PAIR ? static_cast<int>(gridDim.x) >> 1 : static_cast<int>(gridDim.x);
-    allow_next_kernel();   // its CTAs find room as this kernel's CTAs finish: the tails overlap
+    allow_next_kernel();   // its CTAs find room as this kernel's CTAs finish: the tails overlap (and none that holds tensor memory finds any beside one of these)
     constexpr int kWBytes = kTcRows * kTcBlockK * 2;
     extern __shared__ unsigned char raw_shared[];
     unsigned char* tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw_shared) + 1023) & ~static_cast<uintptr_t>(1023));

@@ -88,7 +88,7 @@ moe_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     __shared__ uint32_t tmem_slot;
     __shared__ int failed;
 
-    allow_next_kernel();   // the next product's CTAs fit beside these no more than these beside one another
+    allow_next_kernel();   // the next product's CTAs fit beside these no more than these beside one another, and no other's that hold tensor memory
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kMoeStagesMost; ++s) {

@@ -307,7 +307,7 @@ class Mixer(Part):
     can_defer = False
     # True: its kernels may run at the same time as a feed-forward's on another stream.  What must not happen there: a kernel that lets
     # its successor start early and then waits for tensor memory, while that successor, or the other stream's kernels, hold it.  The products'
-    # kernels cannot get into this (their shared memory admits no more CTAs to a multiprocessor than its tensor memory has room for).
+    # kernels cannot get into this (they have theirs before they let their successor start, or a multiprocessor for themselves).
     can_fork = False
 
     def forward(self, x: torch.Tensor, step: StepInputs, cache: CacheView | None) -> torch.Tensor | None:
