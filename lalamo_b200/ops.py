@@ -2609,11 +2609,17 @@ class Microscaled:
         store = self._store
         if store is not None:
             address = store.data_ptr()
-            return address, address + self._scales_at
-        return self._codes.data_ptr(), self._scales.data_ptr()
+            scales = address + self._scales_at
+        else:
+            address, scales = self._codes.data_ptr(), self._scales.data_ptr()
+        if not (address and scales) and self.rows:
+            raise KernelError(f"{what}: rows without memory")
+        return address, scales
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The numbers, ``[rows, width]``: exact in float32, and in bfloat16 down to its subnormals.  They may be a product's weight at once."""
+        if _modes() or _tracing():
+            _refuse_followed("microscaled_values")
         codes, scales = self._addresses("microscaled_values")
         code = dtype_code(dtype)
         out = (self._store if self._store is not None else self._codes).new_empty((self.rows, self.width), dtype=dtype)
@@ -2634,11 +2640,30 @@ def _check_here(what: str, *tensors: "torch.Tensor | None") -> None:
             raise KernelError(f"{what}: a tensor lies on device {tensor.get_device()}, the current device is {device}")
 
 
-def _refuse_gradients(what: str, *tensors: "torch.Tensor | None") -> None:
-    """Refuses tensors that autograd follows: what comes out would lose their gradients without a word."""
+_forward_ad, _transforms, _modes, _tracing = torch.autograd.forward_ad, torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack, torch._C._is_tracing
+
+
+def _refuse_followed(what: str, *tensors: "torch.Tensor | None") -> None:
+    """Refuses what somebody follows: tensors with gradients or tangents, or in a function transform, and a call that is being traced.  What comes out would lose their gradients,
+    tangents or batches without a word, or become a constant of the trace.  Refuses tensors without memory, too."""
+    gradients = torch.is_grad_enabled()
     for tensor in tensors:
-        if tensor is not None and tensor.requires_grad:
+        if tensor is None:
+            continue
+        if gradients and tensor.requires_grad:
             raise KernelError(f"{what}: there is no backward pass (detach the tensors, or call it under torch.no_grad())")
+        if type(tensor) is not torch.Tensor and isinstance(tensor, torch._subclasses.FakeTensor):
+            raise KernelError(f"{what}: a tensor without memory")
+    if _forward_ad._current_level < 0 and _transforms() is None and not (_modes() or _tracing()):
+        return
+    c = torch._C
+    if c._is_tracing() or c._len_torch_dispatch_stack() > 0 and c._get_dispatch_mode(c._TorchDispatchModeKey.PROXY) is not None:
+        raise KernelError(f"{what}: a trace cannot follow it")
+    tensors = tuple(tensor for tensor in tensors if tensor is not None)
+    if any(c._functorch.is_functorch_wrapped_tensor(tensor) for tensor in tensors):
+        raise KernelError(f"{what}: function transforms cannot follow it")
+    if _forward_ad._current_level >= 0 and any(_forward_ad.unpack_dual(tensor).tangent is not None for tensor in tensors):
+        raise KernelError(f"{what}: it passes no tangents on (give it the primals)")
 
 
 def microscale(x: torch.Tensor, bits: int = 8) -> Microscaled:
@@ -2648,12 +2673,11 @@ def microscale(x: torch.Tensor, bits: int = 8) -> Microscaled:
     NaN as a whole."""
     if bits not in MICROSCALED_BITS:
         raise KernelError(f"microscale: elements have 4 or 8 bits, not {bits}")
+    _refuse_followed("microscale", x)
     _check(x, "x")
     if x.dim() != 2 or x.shape[1] < 1:
         raise KernelError(f"microscale: x must be [rows, width], got {tuple(x.shape)}")
     code = dtype_code(x.dtype)
-    if x.requires_grad and torch.is_grad_enabled():
-        _refuse_gradients("microscale", x)
     rows, width = x.shape
     out = Microscaled._empty(rows, width, bits, x)
     if rows:
@@ -2669,6 +2693,7 @@ def rmsnorm_microscaled(x: torch.Tensor, weight: torch.Tensor, eps: float, *, de
     ``sum_out`` (float32; it may be ``x`` itself) receives the sum.  Rows of up to 32,768 columns."""
     if bits not in MICROSCALED_BITS:
         raise KernelError(f"rmsnorm_microscaled: elements have 4 or 8 bits, not {bits}")
+    _refuse_followed("rmsnorm_microscaled", x, weight, delta, sum_out)
     _check(x, "x", torch.float32)
     _check(weight, "weight", torch.float32)
     shape = x.shape
@@ -2696,8 +2721,6 @@ def rmsnorm_microscaled(x: torch.Tensor, weight: torch.Tensor, eps: float, *, de
     if (x.get_device() != device or weight.get_device() != device or delta is not None and delta.get_device() != device
             or sum_out is not None and sum_out.get_device() != device):
         _check_here("rmsnorm_microscaled", x, weight, delta, sum_out)
-    if torch.is_grad_enabled():
-        _refuse_gradients("rmsnorm_microscaled", x, weight, delta, sum_out)
     out = Microscaled._empty(rows, width, bits, x)
     if rows:
         codes, scales = out._addresses("rmsnorm_microscaled")
@@ -2708,6 +2731,8 @@ def rmsnorm_microscaled(x: torch.Tensor, weight: torch.Tensor, eps: float, *, de
 def linear_microscaled(x: Microscaled, weight: Microscaled, out_dtype: torch.dtype = torch.bfloat16, status: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T`` of the values that microscaled rows stand for: ``x`` in 8 or 4 bits, ``weight`` ``[rows, width]`` in 4; sums of 32 bits, rounded once
     to bfloat16 or handed out as float32.  ``status``: the int32 word in which the kernel reports a wait that gave up."""
+    if _modes() or _tracing():
+        _refuse_followed("linear_microscaled")
     codes, scales = x._addresses("linear_microscaled")
     weight_codes, weight_scales = weight._addresses("linear_microscaled")
     if weight.bits != 4 or weight.width != x.width:
@@ -2729,6 +2754,8 @@ def linear_microscaled(x: Microscaled, weight: Microscaled, out_dtype: torch.dty
 def gated_linear_microscaled(x: Microscaled, up: Microscaled, gate: Microscaled, activation: str, limit: float = 0.0, status: torch.Tensor | None = None) -> Microscaled:
     """``(x @ up.T) * act(x @ gate.T)`` of microscaled rows (8 or 4 bits) and weights (4 bits, ``[hidden, width]`` each), in 8 bits: sums, activation and product
     in 32 bits, then :func:`microscale`'s rule.  ``limit``: of the ``"sigmoid_limit"`` activation.  ``status`` as in :func:`linear_microscaled`."""
+    if _modes() or _tracing():
+        _refuse_followed("gated_linear_microscaled")
     codes, scales = x._addresses("gated_linear_microscaled")
     up_codes, up_scales = up._addresses("gated_linear_microscaled")
     gate_codes, gate_scales = gate._addresses("gated_linear_microscaled")
