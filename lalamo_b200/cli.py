@@ -72,7 +72,7 @@ def generate(
     max_batch_tokens: Annotated[int, Option(help="Tokens one step may run.")] = 2048,
     max_requests: Annotated[int, Option(help="Requests live at a time.")] = 64,
     chunk_size: Annotated[Optional[int], Option(help="Longest portion of one prompt in a step.", show_default="max-batch-tokens")] = None,
-    microscaled_feed_forward: Annotated[bool, Option("--microscaled-feed-forward", help="Hold the gated feed-forwards' weights in 4 bits (microscaled) and their rows in 8.")] = False,
+    microscaled_feed_forward: Annotated[bool, Option("--microscaled-feed-forward", help="Hold the gated feed-forwards' weights in 4 bits (microscaled) and their rows in 8; routed experts and dense feed-forwards stay as they are, and a model without a gated one is refused.")] = False,
     stats: Annotated[bool, Option(help="Print scheduler statistics to standard error.")] = False,
 ) -> None:
     from dataclasses import replace

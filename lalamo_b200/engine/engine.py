@@ -52,7 +52,9 @@ class EngineConfig:
     max_batch_tokens: int = 2048  # tokens one step may run (the scheduler's budget)
     device: str = "cuda:0"
     cuda_graphs: bool = True  # replay decode steps from CUDA graphs
-    microscaled_feed_forward: bool = False  # gated feed-forwards' weights in 4 bits with a scale per 32, their rows in 8 (bfloat16 engines)
+    # gated feed-forwards' weights in 4 bits with a scale per 32, their rows in 8 (bfloat16 engines); also one that stands beside routed experts, while the experts
+    # and dense feed-forwards stay as they are.  A model without a gated one is refused
+    microscaled_feed_forward: bool = False
     freeze_gc: bool = True  # after loading, exempt the objects alive so far from garbage collection passes
     poison_freed: bool = False  # tests: overwrite pages and state slots with NaN when they are given back
 

@@ -22,7 +22,7 @@ import torch
 
 from .base import CacheNeed, CacheView, CompositeNeed, CompositeView, FeedForward, Mixer, Norm, Part, Runtime, StepInputs, TensorDecl, build_part, part_type
 
-__all__ = ["Block", "HyperBlock", "OutputNormBlock", "ParallelBlock", "PreNormBlock", "SandwichNormBlock", "block_tensor_decls", "block_type", "build_block", "register_arrangement"]
+__all__ = ["Block", "HyperBlock", "OutputNormBlock", "ParallelBlock", "PreNormBlock", "SandwichNormBlock", "block_part_specs", "block_tensor_decls", "block_type", "build_block", "register_arrangement"]
 
 # A parallel block's sublayers on two streams (LALAMO_B200_PARALLEL_STREAMS=0: one after the other).
 PARALLEL_STREAMS = os.environ.get("LALAMO_B200_PARALLEL_STREAMS", "1") != "0"
@@ -49,6 +49,11 @@ def block_type(spec: Any) -> type["Block"]:
 def _role_specs(spec: Any) -> list[tuple[str, Any]]:
     """The part specifications of a layer, by role; roles whose field is ``None`` are left out."""
     return [(role, getattr(spec, role)) for role in block_type(spec).roles if getattr(spec, role, None) is not None]
+
+
+def block_part_specs(spec: Any) -> list[Any]:
+    """The part specifications of a layer."""
+    return [part_spec for _, part_spec in _role_specs(spec)]
 
 
 def block_tensor_decls(spec: Any) -> dict[tuple[str, str], TensorDecl]:

@@ -1,7 +1,7 @@
 """Dense gated feed-forward (``lalamo/modules/mlp.py:233-262``): ``down(up(x) * act(gate(x)))``
 with the up and gate projections fused into one product, rows ordered ``[up ; gate]``.  Where the engine
 asks for it (``Runtime.microscaled_feed_forward``) the gated one holds its weights in 4 bits and reads and hands on rows of 8
-(``ops.Microscaled``)."""
+(``ops.Microscaled``); the dense one, and routed experts, do not change."""
 
 from __future__ import annotations
 

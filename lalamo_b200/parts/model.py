@@ -12,10 +12,10 @@ from typing import Mapping
 import torch
 
 from .. import ops
-from ..config.plan import ModelPlan
+from ..config.plan import GatedMLPSpec, ModelPlan
 from .base import BorrowedKVNeed, CacheNeed, CacheView, CompositeNeed, Norm, Part, Runtime, StepInputs, TensorDecl, build_part, part_type
 from .embedding import Embedding, Head
-from .block import Block, block_tensor_decls, build_block
+from .block import Block, block_part_specs, block_tensor_decls, build_block
 
 __all__ = ["DecoderModel", "plan_tensor_decls"]
 
@@ -47,8 +47,15 @@ def _borrows(need: CacheNeed | None) -> bool:
     return isinstance(need, BorrowedKVNeed)
 
 
+def _has_gated_feed_forward(plan: ModelPlan) -> bool:
+    """Whether a layer has a gated feed-forward, by itself or beside routed experts."""
+    return any(isinstance(spec, GatedMLPSpec) or isinstance(getattr(spec, "shared", None), GatedMLPSpec) for layer in plan.layers for spec in block_part_specs(layer))
+
+
 class DecoderModel:
     def __init__(self, plan: ModelPlan, tensors: Mapping[TensorKey, torch.Tensor], runtime: Runtime) -> None:
+        if runtime.microscaled_feed_forward and not _has_gated_feed_forward(plan):
+            raise ValueError("microscaled feed-forwards: the model has no gated feed-forward to hold so (routed experts and dense feed-forwards are none)")
         self.plan = plan
         self.runtime = runtime
         embedding_tensors = {local: tensor for (path, local), tensor in tensors.items() if path == ("embedding",)}
