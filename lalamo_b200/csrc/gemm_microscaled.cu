@@ -949,26 +949,50 @@ inline TokenTiles cut_tokens(int tokens, long long row_tiles, int walkers, long 
 
 // Which kernel.  Few tiles are cut along K: up to 128 tokens, and up to half of the multiprocessors in tiles of 128 x 128.  Else the tiles are walked, by pairs of CTAs where
 // those are sooner done although they start some 2.5 us later.
+enum MsKernel { kMsShared, kMsWalked, kMsPairs };
+struct MsChoice {
+    MsKernel kernel;
+    TokenTiles cut;   // of the walked ones
+};
+template <int BITS, bool GATED>
+MsChoice choose_microscaled(int tokens, int n, int chunks) {
+    const long long row_tiles = GATED ? (n + 127) / 128 * 2 : (n + kMsRows - 1) / kMsRows;
+    const int sms = multiprocessor_count();
+    if (tokens <= 128 || row_tiles * ((tokens + 127) / 128) <= sms / 2) return {kMsShared, {}};
+    const long long stages = (chunks + MsShape<BITS, 128>::kChunks - 1) / MsShape<BITS, 128>::kChunks;
+    const TokenTiles alone = cut_tokens(tokens, row_tiles, sms, stages, BITS == 8 ? 29 : 30, 36);
+    if constexpr (BITS == 8 && !GATED) {
+        const TokenTiles pairs = cut_tokens(tokens, (row_tiles + 1) / 2, sms / 2, stages, 27, 32);
+        if (pairs.cost + 250 < alone.cost) return {kMsPairs, pairs};
+    }
+    return {kMsWalked, alone};
+}
+
 template <int BITS, bool GATED>
 int launch_microscaled_tiles(const void* x, const void* w, const void* gate, const MsParams& p, cudaStream_t stream) {
-    const long long row_tiles = GATED ? p.out_chunks * 2 : (p.n + kMsRows - 1) / kMsRows;
-    const int sms = multiprocessor_count();
-    if (p.tokens <= 16) return launch_microscaled_split<BITS, 16, GATED>(x, w, gate, p, stream);
-    if (p.tokens <= 32) return launch_microscaled_split<BITS, 32, GATED>(x, w, gate, p, stream);
-    if (p.tokens <= 64) return launch_microscaled_split<BITS, 64, GATED>(x, w, gate, p, stream);
-    if (p.tokens <= 128 || row_tiles * ((p.tokens + 127) / 128) <= sms / 2) return launch_microscaled_split<BITS, 128, GATED>(x, w, gate, p, stream);
-    const long long stages = (p.chunks + MsShape<BITS, 128>::kChunks - 1) / MsShape<BITS, 128>::kChunks;
-    const TokenTiles alone = cut_tokens(p.tokens, row_tiles, sms, stages, BITS == 8 ? 29 : 30, 36);
-    if constexpr (BITS == 8 && !GATED) {
-        const TokenTiles pairs = cut_tokens(p.tokens, (row_tiles + 1) / 2, sms / 2, stages, 27, 32);
-        if (pairs.cost + 250 < alone.cost) return launch_microscaled<BITS, GATED, true>(x, w, gate, p, pairs.count, pairs.wide, stream);
+    const MsChoice choice = choose_microscaled<BITS, GATED>(p.tokens, p.n, p.chunks);
+    if (choice.kernel == kMsShared) {
+        if (p.tokens <= 16) return launch_microscaled_split<BITS, 16, GATED>(x, w, gate, p, stream);
+        if (p.tokens <= 32) return launch_microscaled_split<BITS, 32, GATED>(x, w, gate, p, stream);
+        if (p.tokens <= 64) return launch_microscaled_split<BITS, 64, GATED>(x, w, gate, p, stream);
+        return launch_microscaled_split<BITS, 128, GATED>(x, w, gate, p, stream);
     }
-    return launch_microscaled<BITS, GATED, false>(x, w, gate, p, alone.count, alone.wide, stream);
+    if constexpr (BITS == 8 && !GATED) {
+        if (choice.kernel == kMsPairs) return launch_microscaled<BITS, GATED, true>(x, w, gate, p, choice.cut.count, choice.cut.wide, stream);
+    }
+    return launch_microscaled<BITS, GATED, false>(x, w, gate, p, choice.cut.count, choice.cut.wide, stream);
 }
 
 }  // namespace lb
 
 extern "C" {
+
+// Which kernel runs a product of these sizes on the current device: 0 tiles whose K is shared out, 1 walked tiles, 2 by pairs of CTAs; -2 for sizes that none takes.
+int lb_microscaled_kernel(int tokens, int n, int chunks, int bits, int gated) {
+    if (tokens < 1 || tokens > lb::kMsMostRows || n < 1 || n > lb::kMsMostRows || chunks < 1 || chunks > (1 << 22) || (bits != 4 && bits != 8)) return -2;
+    if (gated) return bits == 8 ? lb::choose_microscaled<8, true>(tokens, n, chunks).kernel : lb::choose_microscaled<4, true>(tokens, n, chunks).kernel;
+    return bits == 8 ? lb::choose_microscaled<8, false>(tokens, n, chunks).kernel : lb::choose_microscaled<4, false>(tokens, n, chunks).kernel;
+}
 
 // out [tokens, n] = x w^T, bfloat16 or float32.  x [tokens, 128 * chunks] in `bits` bits, w [n, 128 * chunks] in 4.
 // Returns 0, a CUDA error, -2 for sizes or addresses that the kernel does not take, -5 if no tensor map could be made.

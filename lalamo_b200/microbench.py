@@ -99,7 +99,7 @@ def microscaled(arguments: argparse.Namespace) -> dict:
 
     microseconds = _time(run_all, arguments.repeats, arguments.graph) / len(weights)
     products = 2 if arguments.epilogue == "gated" else 1
-    return {"kernel": "microscaled product", "tokens": tokens, "rows": rows, "width": width, "bits": arguments.bits, "epilogue": arguments.epilogue, "us": round(microseconds, 2),
+    return {"kernel": f"microscaled product, {ops.microscaled_kernel(tokens, rows, width, arguments.bits, arguments.epilogue == 'gated')}", "tokens": tokens, "rows": rows, "width": width, "bits": arguments.bits, "epilogue": arguments.epilogue, "us": round(microseconds, 2),
             "tflops": round(2 * products * tokens * rows * width / microseconds / 1e6, 1), "weight_gb_per_s": round(products * rows * width * 17 / 32 / microseconds / 1e3, 1)}
 
 

@@ -2728,6 +2728,15 @@ def rmsnorm_microscaled(x: torch.Tensor, weight: torch.Tensor, eps: float, *, de
     return out
 
 
+def microscaled_kernel(tokens: int, rows: int, width: int, bits: int, gated: bool = False) -> str:
+    """The kernel that :func:`linear_microscaled` (or the gated product) launches for these sizes: ``"shared"``, tiles whose K several CTAs may share out, ``"walked"``, a CTA a
+    multiprocessor going from tile to tile, or ``"pairs"``, two CTAs to a tile."""
+    code = _lib().lb_microscaled_kernel(tokens, rows, -(-width // 128), bits, 1 if gated else 0)
+    if code < 0:
+        raise KernelError(f"microscaled_kernel: no kernel takes {tokens} rows of {width} elements in {bits} bits and a weight of {rows}")
+    return ("shared", "walked", "pairs")[code]
+
+
 def linear_microscaled(x: Microscaled, weight: Microscaled, out_dtype: torch.dtype = torch.bfloat16, status: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T`` of the values that microscaled rows stand for: ``x`` in 8 or 4 bits, ``weight`` ``[rows, width]`` in 4; sums of 32 bits, rounded once
     to bfloat16 or handed out as float32.  ``status``: the int32 word in which the kernel reports a wait that gave up."""
