@@ -47,3 +47,11 @@ def test_the_sizes_are_the_sources():
     assert "kPersistSharedBytes = 4 * 48 * 1024 + kPersistExchangeBytes + 1024 + 256" in (folder / "gemm_tcgen05.cu").read_text()
     moe = (folder / "moe_tcgen05.cu").read_text()
     assert "kMoeStageArea = 196608" in moe and "kMoePitch = 80" in moe and "most = 1024 + kMoeStageArea + 2 * kMoeRows * kMoePitch + 2 * (kMoeMaxExperts + 1) * 4" in moe
+
+
+def test_loads_of_tensor_memory_hold_their_wait():
+    """What a load of sixteen columns brings is there when its statement ends: with the wait in a statement of its own, whatever only uses the values may be placed between the two."""
+    text = (Path(native.source_files()[0]).parent / "tcgen05.cuh").read_text()
+    body = text[text.index("void tmem_load_16(") :]
+    body = body[: body.index("\n}")]
+    assert body.count("asm volatile") == 1 and body.index("tcgen05.ld.") < body.index("tcgen05.wait::ld")
