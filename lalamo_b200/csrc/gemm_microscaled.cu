@@ -893,14 +893,15 @@ int launch_microscaled_split(const void* x, const void* w, const void* gate, MsP
     p.bulk_store = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 ? 1 : 0;
     const int row_tiles = GATED ? p.out_chunks * 2 : (p.n + kMsRows - 1) / kMsRows, token_tiles = (p.tokens + BN - 1) / BN, sms = multiprocessor_count();
     const int stages = (p.chunks + MsShape<BITS, BN>::kChunks - 1) / MsShape<BITS, BN>::kChunks;
-    // Two CTAs fit a multiprocessor: clusters of eight that have one each do not all find room at once (2048 x 8192 and a token: 9.1 us, and 5.0 with room for two),
-    // and a deeper ring gains nothing.  A stage takes 0.18 us, a meeting of up to four CTAs 0.6 us and of eight 1.2, more with more tokens: beyond four where each still has
-    // three stages (8 tokens, 2048 x 2048: 3.4 us by four, 3.8 by eight; 1024 x 4608 4.6 and 3.9), and of more than 32 tokens six at most (128 tokens, 2048 x 8192: 10.5 us by
-    // four, 9.6 by six, 11.3 by eight).
+    // Two CTAs fit a multiprocessor: clusters of eight that have one each do not all find room at once (2048 x 8192 and a token: 9.1 us, and 5.2 with room for two),
+    // and a deeper ring gains nothing.  A stage takes 0.18 us, the meetings of up to four CTAs 1.0 us and of eight 1.6, more with more tokens: beyond four where each still has
+    // three stages (8 tokens, rows of 4 bits, 2048 x 2048: 3.2 us by four, 3.8 by eight; of 8 bits, 1024 x 4608 4.8 and 4.2), and of more than 32 tokens six at most (128 tokens,
+    // 2048 x 8192: 11.4 us by four, 10.6 by six, 12.9 by eight).
     int wanted = max(1, min(min(sms / (row_tiles * token_tiles), stages), min(max(4, stages / 3), BN > 32 ? 6 : kMsLargestSplit)));
-    // Gated tiles that nearly fill the multiprocessors are cut in two all the same, two CTAs to each (8192 x 2048, 64 tokens: 11.3 and 9.4 us; other products lose
-    // by it: 6.4 and 7.3).
-    if (GATED && wanted == 1 && stages > 1 && row_tiles * token_tiles <= sms && (BITS == 8 || BN > 16)) wanted = 2;
+    // Gated tiles that nearly fill the multiprocessors are cut in two all the same, two CTAs to each, where that saves each more than four stages or there are many tokens: 8192 x
+    // 8192, 16 tokens 17.5 us and 21.5, 8192 x 1024, 128 tokens 10.1 and 10.9; with few of both the meetings cost more: 8192 x 1024, 8 tokens 5.0 us and 4.5, rows of 4 bits, 2048
+    // columns, 6.2 and 5.2.  (Other products lose by it, 6.4 us and 7.3.)
+    if (GATED && wanted == 1 && stages > (BN > 64 ? 1 : 8) && row_tiles * token_tiles <= sms) wanted = 2;
     const int per_split = (stages + wanted - 1) / wanted, splits = (stages + per_split - 1) / per_split;   // each has a stage at least
     const int ring = min(per_split, MsSplit<BITS, BN>::kMostStages);
     auto kernel = gemm_microscaled_split_kernel<BITS, BN, GATED>;

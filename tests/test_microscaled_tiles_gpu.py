@@ -28,7 +28,7 @@ def check_product(tokens, rows, width, bits):
 @pytest.mark.parametrize("tokens", [1, 7, 16, 17, 40, 64, 65, 128])
 @pytest.mark.parametrize("hidden,width", [(8192, 2048), (4800, 300), (9400, 1001)])
 def test_gated_products_cut_in_two(tokens, hidden, width, bits):
-    """75 to 148 tiles of 64 rows of each weight: too many for the multiprocessors to share out, and cut in two all the same (but rows of 4 bits with up to 16 tokens).  Up times gate as
+    """75 to 148 tiles of 64 rows of each weight: too many for the multiprocessors to share out, and cut in two all the same where K is long or the tokens are many.  Up times gate as
     in the tests of fewer tiles: few columns are not zero, so that the product of the two sums is exact."""
     assert 75 <= -(-hidden // 128) * 2 <= 148
     assert ops.microscaled_kernel(tokens, hidden, width, bits, gated=True) == "shared"
