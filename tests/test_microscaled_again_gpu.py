@@ -80,3 +80,24 @@ def test_rows_and_norms(tokens, width, bits):
         calls.append(lambda x=x, half=half, weight=weight: ops.rmsnorm_microscaled(x, weight, 1e-5, delta=half, sum_out=torch.empty_like(x), bits=bits))
         calls.append(lambda x=x, delta=delta, weight=weight: ops.rmsnorm_microscaled(x, weight, 1e-5, delta=delta, bits=bits).values(torch.float32))
     check_again(calls, 10)
+
+
+@pytest.mark.parametrize("tokens", [(20, 64), (33, 128), (100, 17), (1, 600)])
+def test_beside_bfloat16_products(tokens):
+    """Streams of bfloat16 and microscaled products in turn, K short and many tiles: all of them want tensor memory, and start early behind one another."""
+    count, status = len(tokens), torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    x = [torch.randn(t, 256, device=DEVICE).to(torch.bfloat16) for t in tokens]
+    weight, small = torch.randn(4096, 256, device=DEVICE).to(torch.bfloat16), rows_of(20000, 128, 4, 1)
+    rows = [rows_of(t, 128, 8, t) for t in tokens]
+    want = [(ops.linear(x[k], weight, status=status), ops.linear_microscaled(rows[k], small, status=status)) for k in range(count)]
+    streams = [torch.cuda.Stream() for _ in range(count)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(40):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got.append((k, ops.linear(x[k], weight, status=status), ops.linear_microscaled(rows[k], small, status=status)))
+    torch.cuda.synchronize()
+    assert status.item() == 0
+    for k, one, other in got:
+        assert torch.equal(one, want[k][0]) and torch.equal(other, want[k][1])
