@@ -4,7 +4,7 @@
     python -m lalamo_b200.microbench prefill-attention --tokens 2048 [--kernel mma] [--last-tiles 1]
     python -m lalamo_b200.microbench decode-attention --batch 8 --context 4096
     python -m lalamo_b200.microbench microscaled --tokens 8 --rows 8192 --width 2048 --epilogue gated [--bits 4] --graph
-    python -m lalamo_b200.microbench step-kernels --tokens 2048 [--preset lfm2-1.2b] [--batch 8 --context 4096]
+    python -m lalamo_b200.microbench step-kernels --tokens 2048 [--preset lfm2-1.2b] [--batch 8 --context 4096] [--microscaled-feed-forward]
 
 Each prints one JSON line.  Sizes default to the LFM2-1.2B shape (32 query heads over 8 K/V heads
 of 64 channels, pages of 16 keys).  ``linear`` rotates over several weight matrices; with
@@ -168,7 +168,7 @@ def step_kernels(arguments: argparse.Namespace) -> dict:
     """The kernels of one step with their durations while the step runs as it does in production (warm
     caches, launches overlapping, recorded graphs), as CUPTI reports them through ``torch.profiler``: a
     prompt of ``--tokens`` tokens in one step, or with ``--batch`` a decode step of that many requests at
-    ``--context``."""
+    ``--context``; and the median time of a call of the engine's step by itself, between events around it (the host's work before its launches included)."""
     import numpy as np
     from torch.profiler import ProfilerActivity, profile
 
@@ -181,7 +181,7 @@ def step_kernels(arguments: argparse.Namespace) -> dict:
     room = arguments.batch * (arguments.context + 64) if decode else tokens + 64
     engine = Engine.random(config_from_dict(PRESETS[arguments.preset]), seed=1, std=0.02,
                            engine_config=EngineConfig(dtype="bfloat16", page_size=16, max_tokens=room, max_requests=max(1, arguments.batch),
-                                                      max_batch_tokens=max(tokens, 2048), cuda_graphs=True))
+                                                      max_batch_tokens=max(tokens, 2048), cuda_graphs=True, microscaled_feed_forward=arguments.microscaled_feed_forward))
     random = np.random.default_rng(0)
     if decode:
         names = list(range(arguments.batch))
@@ -190,24 +190,32 @@ def step_kernels(arguments: argparse.Namespace) -> dict:
             engine.cache.reserve(name, arguments.context - 8)
             engine.cache.commit(name, arguments.context - 8)
 
-        def one() -> None:
-            engine.step([StepEntry(name, [int(random.integers(0, engine.vocab_size))], [0]) for name in names])
-            torch.cuda.synchronize()
+        def one() -> float:
+            return timed([StepEntry(name, [int(random.integers(0, engine.vocab_size))], [0]) for name in names])
     else:
-        def one() -> None:
+        def one() -> float:
             engine.admit("prompt")
-            engine.step([StepEntry("prompt", random.integers(0, engine.vocab_size, size=tokens).tolist(), [tokens - 1])])
-            torch.cuda.synchronize()
+            milliseconds = timed([StepEntry("prompt", random.integers(0, engine.vocab_size, size=tokens).tolist(), [tokens - 1])])
             engine.release("prompt")
+            return milliseconds
 
-    for _ in range(3):
-        one()
+    def timed(entries: list) -> float:
+        begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        begin.record()
+        engine.step(entries)
+        end.record()
+        torch.cuda.synchronize()
+        return begin.elapsed_time(end)
+
+    # (as many as keep the requests within the pages kept for them)
+    milliseconds = sorted(one() for _ in range(48))[24]
     with profile(activities=[ProfilerActivity.CUDA]) as session:
         one()
     rows = [(event.key, event.count, event.device_time_total) for event in session.key_averages() if event.device_time_total > 0]
     rows.sort(key=lambda row: -row[2])
     total = sum(row[2] for row in rows)
     return {"step": f"decode batch {arguments.batch} context {arguments.context}" if decode else f"prompt of {tokens} tokens", "preset": arguments.preset,
+            "microscaled_feed_forward": arguments.microscaled_feed_forward, "ms_step": round(milliseconds, 4),
             "us_total": round(total, 1), "kernels": [{"name": name[:90], "launches": count, "us": round(time, 1), "us_each": round(time / count, 2)} for name, count, time in rows]}
 
 
@@ -258,6 +266,7 @@ def main(argv: list[str] | None = None) -> int:
     one.add_argument("--batch", type=int, default=0, help="a decode step of this many requests instead of a prompt")
     one.add_argument("--context", type=int, default=4096)
     one.add_argument("--preset", default="lfm2-1.2b")
+    one.add_argument("--microscaled-feed-forward", action="store_true", help="gated feed-forwards in 4 bits")
     one.set_defaults(function=step_kernels)
     arguments = parser.parse_args(argv)
     if not torch.cuda.is_available():
