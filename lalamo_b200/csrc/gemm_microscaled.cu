@@ -133,8 +133,8 @@ struct MsShape {
     static constexpr uint32_t kWCounted = BITS == 8 ? kWBytes / 2 : kWBytes;
 };
 
-// A landed stage's scales to a set of columns of tensor memory.  The whole warp comes here, and a lane is elected for every instruction (gated 8192 x 2048, 8 tokens:
-// 6.5 us, and 7.1 with one lane for all of a stage); for a pair one lane comes, elected for all of them (4,096 tokens, 2048 x 8192: 61 us, and 96 with one each).
+// A landed stage's scales to a set of columns of tensor memory.  The whole warp comes here, and a lane is elected for every instruction (gated 8192 x 2048 from L2, 8 tokens:
+// 6.5 us, and 7.1 with one lane for all of a stage, both before the clusters' last meeting ordered the reads); for a pair one lane comes, elected for all of them (4,096 tokens, 2048 x 8192: 61 us, and 96 with one each).
 template <typename Shape, bool PAIR>
 __device__ __forceinline__ void copy_stage_scales(const unsigned char* stage, uint32_t columns, int chunks) {
     const unsigned char* scales = stage + Shape::kWBytes + Shape::kXBytes;

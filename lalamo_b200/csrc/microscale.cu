@@ -43,7 +43,7 @@ template <typename T>
 struct MicroscaleShape {
     static constexpr int kCount = sizeof(T) == 2 ? 16 : 8, kLanes = 128 / kCount, kRounds = sizeof(T) == 2 ? 2 : 1;
 };
-// The same of the values' kernel: eight columns, four times of bfloat16 (14.9 us, 6.8 TB/s; once 19.9), once of float32 (32.0 us; four times 36.4).
+// The same of the values' kernel: eight columns, four times of bfloat16 (14.9 us, 6.8 TB/s; once 19.9), once of float32 (32.0 us; four times 36.4), without the launch behind it.
 template <typename T>
 constexpr int kValuesRounds = sizeof(T) == 2 ? 4 : 1;
 
