@@ -963,8 +963,8 @@ MsChoice choose_microscaled(int tokens, int n, int chunks) {
     const long long stages = (chunks + MsShape<BITS, 128>::kChunks - 1) / MsShape<BITS, 128>::kChunks;
     const TokenTiles alone = cut_tokens(tokens, row_tiles, sms, stages, BITS == 8 ? 29 : 30, 36);
     if constexpr (BITS == 8 && !GATED) {
-        const TokenTiles pairs = cut_tokens(tokens, (row_tiles + 1) / 2, sms / 2, stages, 27, 32);
-        if (pairs.cost + 250 < alone.cost) return {kMsPairs, pairs};
+        const TokenTiles pairs = cut_tokens(tokens, (row_tiles + 1) / 2, max(1, sms / 2), stages, 27, 32);
+        if (sms > 1 && pairs.cost + 250 < alone.cost) return {kMsPairs, pairs};
     }
     return {kMsWalked, alone};
 }
@@ -988,9 +988,12 @@ int launch_microscaled_tiles(const void* x, const void* w, const void* gate, con
 
 extern "C" {
 
-// Which kernel runs a product of these sizes on the current device: 0 tiles whose K is shared out, 1 walked tiles, 2 by pairs of CTAs; -2 for sizes that none takes.
+// Which kernel runs a product of these sizes on the current device: 0 tiles whose K is shared out, 1 walked tiles, 2 by pairs of CTAs; -2 for sizes that none takes,
+// -3 without a device.
 int lb_microscaled_kernel(int tokens, int n, int chunks, int bits, int gated) {
     if (tokens < 1 || tokens > lb::kMsMostRows || n < 1 || n > lb::kMsMostRows || chunks < 1 || chunks > (1 << 22) || (bits != 4 && bits != 8)) return -2;
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return -3;
     if (gated) return bits == 8 ? lb::choose_microscaled<8, true>(tokens, n, chunks).kernel : lb::choose_microscaled<4, true>(tokens, n, chunks).kernel;
     return bits == 8 ? lb::choose_microscaled<8, false>(tokens, n, chunks).kernel : lb::choose_microscaled<4, false>(tokens, n, chunks).kernel;
 }

@@ -2732,6 +2732,8 @@ def microscaled_kernel(tokens: int, rows: int, width: int, bits: int, gated: boo
     """The kernel that :func:`linear_microscaled` (or the gated product) launches for these sizes: ``"shared"``, tiles whose K several CTAs may share out, ``"walked"``, a CTA a
     multiprocessor going from tile to tile, or ``"pairs"``, two CTAs to a tile."""
     code = _lib().lb_microscaled_kernel(tokens, rows, -(-width // 128), bits, 1 if gated else 0)
+    if code == -3:
+        raise KernelError("microscaled_kernel: there is no CUDA device")
     if code < 0:
         raise KernelError(f"microscaled_kernel: no kernel takes {tokens} rows of {width} elements in {bits} bits and a weight of {rows}")
     return ("shared", "walked", "pairs")[code]

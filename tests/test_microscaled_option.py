@@ -60,3 +60,16 @@ def test_the_flag(monkeypatch):
         result = CliRunner().invoke(app, ["generate", "--random-weights", "3", "--preset", "lfm2-1.2b", "--prompt-ids", "1 2", "--dtype", "bfloat16", *flag])
         assert result.exit_code != 0
     assert [config.microscaled_feed_forward for config in seen] == [False, True]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="without a device")
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_which_kernel_without_a_device(bits, gated):
+    from lalamo_b200 import ops
+
+    for tokens in (1, 4096):
+        with pytest.raises(ops.KernelError, match="device"):
+            ops.microscaled_kernel(tokens, 2048, 8192, bits, gated)
+    with pytest.raises(ops.KernelError, match="no kernel"):
+        ops.microscaled_kernel(0, 2048, 8192, bits, gated)
