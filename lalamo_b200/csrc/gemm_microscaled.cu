@@ -725,6 +725,7 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
     const auto has_read = [&]() {
         if (arrived) return;
         arrived = true;
+        __syncwarp();   // the lanes may have parted where the pass before wrote
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     };
     if constexpr (!GATED) {
@@ -790,6 +791,7 @@ gemm_microscaled_split_kernel(const __grid_constant__ CUtensorMap map_w, const _
         }
     }
     has_read();   // a warp that had no tokens
+    __syncwarp();
     if (splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 

@@ -26,3 +26,12 @@ def test_arrivals_order_what_was_read(path):
 
 def test_there_are_meetings():
     assert any("barrier.cluster.arrive" in code_of(path) for path in SOURCES)
+
+
+def test_warps_that_may_have_parted_meet_first():
+    """The aligned forms want a warp's lanes together; behind writes that only some lanes make they may not be."""
+    code = code_of(next(path for path in SOURCES if path.name == "gemm_microscaled.cu"))
+    found = [match.start() for match in re.finditer(r'asm volatile\("barrier\.cluster\.(arrive|wait)', code)]
+    assert len(found) == 2
+    for place in found:
+        assert "__syncwarp();" in code[place - 120 : place]
